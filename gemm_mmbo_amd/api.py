@@ -10,7 +10,9 @@ There is no CPU path: if the HIP library has not been built this module raises o
 import ctypes
 import os
 
-F32, F16, F64 = 0, 1, 2
+F32, F16, F64, BF16 = 0, 1, 2, 3                # (BF16: 4-bit weights and the mixture of experts only)
+MOE_SOFTMAX, MOE_SIGMOID = 0, 1
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 512, 512, 32
 OP_N, OP_T = 0, 1
 CONFIG_AUTO = -1
 
@@ -19,6 +21,7 @@ LIB_PATH = os.path.join(_HERE, "csrc", "libmmbo_gemm.so")
 
 EXPORTS = (
     "mmbo_gemm", "mmbo_gemm_strided_batched", "mmbo_gemm_strided_batched_static_workspace", "mmbo_static_workspace_bytes",
+    "mmbo_gemm_w4", "mmbo_w4_quantize", "mmbo_w4_dequantize", "mmbo_moe_workspace_bytes", "mmbo_moe",
     "mmbo_num_configs", "mmbo_config_info", "mmbo_select_config", "mmbo_auto_info",
     "mmbo_wg_remap", "mmbo_chip_block_remap", "mmbo_batch_xcd_remap", "mmbo_release_workspace", "mmbo_release_stream_workspace", "mmbo_workspace_info",
     "mmbo_probe_mfma_ceiling", "mmbo_probe_stream", "mmbo_status_string", "mmbo_last_hip_error", "mmbo_version",
@@ -40,6 +43,19 @@ class ConfigDesc(ctypes.Structure):
         d = {f: getattr(self, f) for f, _ in self._fields_}
         d["name"] = self.name.decode()
         return d
+
+
+class MoeMatrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("ld", ctypes.c_size_t), ("stride", ctypes.c_longlong), ("scales", ctypes.c_void_p),
+                ("lds", ctypes.c_size_t), ("stride_scales", ctypes.c_longlong), ("zeros", ctypes.c_void_p), ("ldz", ctypes.c_size_t),
+                ("stride_zeros", ctypes.c_longlong)]
+
+
+class MoeLayer(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("router_dtype", ctypes.c_int), ("scoring", ctypes.c_int), ("renormalize", ctypes.c_int),
+                ("hidden", ctypes.c_size_t), ("inner", ctypes.c_size_t), ("experts", ctypes.c_size_t), ("top_k", ctypes.c_size_t),
+                ("group", ctypes.c_size_t), ("router", ctypes.c_void_p), ("ld_router", ctypes.c_size_t), ("bias", ctypes.c_void_p),
+                ("gate_up", MoeMatrix), ("down", MoeMatrix)]
 
 
 _lib = None
@@ -74,6 +90,16 @@ def lib():
         L.mmbo_gemm_strided_batched_static_workspace.argtypes = L.mmbo_gemm_strided_batched.argtypes
         L.mmbo_gemm_strided_batched_static_workspace.restype = ci
         L.mmbo_static_workspace_bytes.restype = sz
+        L.mmbo_gemm_w4.argtypes = [ci, sz, sz, sz, sz, vp, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp]
+        L.mmbo_gemm_w4.restype = ci
+        L.mmbo_w4_quantize.argtypes = [ci, ci, sz, sz, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp]
+        L.mmbo_w4_quantize.restype = ci
+        L.mmbo_w4_dequantize.argtypes = [ci, sz, sz, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp]
+        L.mmbo_w4_dequantize.restype = ci
+        L.mmbo_moe_workspace_bytes.argtypes = [ctypes.POINTER(MoeLayer), sz]
+        L.mmbo_moe_workspace_bytes.restype = sz
+        L.mmbo_moe.argtypes = [ctypes.POINTER(MoeLayer), sz, vp, vp, sz, vp, vp, sz, vp, vp, vp, sz, vp]
+        L.mmbo_moe.restype = ci
         L.mmbo_num_configs.argtypes = [ci]
         L.mmbo_num_configs.restype = ci
         L.mmbo_config_info.argtypes = [ci, ci, ctypes.POINTER(ConfigDesc)]
@@ -172,6 +198,59 @@ if _frontend is not None:
     _frontend.setup(*_PYTHON_FRONT_ENDS, _check)
     gemm, gemm_strided_batched = _frontend.gemm, _frontend.gemm_strided_batched
     gemm_strided_batched_static_workspace = _frontend.gemm_strided_batched_static_workspace
+
+
+def gemm_w4(dtype, m, n, k, group, alpha, Q, ldq, scales, lds, zeros, ldz, B, ldb, beta, C, ldc, stream=None):
+    """C = alpha*W*B + beta*C with W of m rows and k columns in 4 bits (the format: include/mmbo_gemm.h): codes Q, ldq codes from row to row, a
+    scale and a zero point (zeros None: 8) for every `group` codes of a row.  dtype F16 or BF16: scales, B, C."""
+    al, be = _scalars(F32, alpha, beta)
+    _check(lib().mmbo_gemm_w4(dtype, m, n, k, group, ctypes.byref(al), _devptr(Q), ldq, _devptr(scales), lds, _devptr(zeros), ldz,
+                              _devptr(B), ldb, ctypes.byref(be), _devptr(C), ldc, _stream_handle(stream)))
+
+
+def w4_quantize(w_dtype, dtype, m, k, group, W, ldw, Q, ldq, scales, lds, zeros=None, ldz=0, stream=None):
+    """W (F32, F16 or BF16; row i at W + i*ldw) to 4 bits, by rounding to nearest; with `zeros` each group's range need not be symmetric."""
+    _check(lib().mmbo_w4_quantize(w_dtype, dtype, m, k, group, _devptr(W), ldw, _devptr(Q), ldq, _devptr(scales), lds, _devptr(zeros), ldz,
+                                  _stream_handle(stream)))
+
+
+def w4_dequantize(dtype, m, k, group, Q, ldq, scales, lds, zeros, ldz, W, ldw, stream=None):
+    """4-bit weights back to dtype: W[l + i*ldw] = (code - zero) * scale."""
+    _check(lib().mmbo_w4_dequantize(dtype, m, k, group, _devptr(Q), ldq, _devptr(scales), lds, _devptr(zeros), ldz, _devptr(W), ldw,
+                                    _stream_handle(stream)))
+
+
+def moe_matrix(data, ld, stride, scales=None, lds=0, stride_scales=0, zeros=None, ldz=0, stride_zeros=0):
+    """One weight of all experts, for moe_layer(): `ld` elements from row to row, `stride` from expert to expert (4-bit weights: codes, and their
+    scales and zero points).  It holds on to the tensors."""
+    w = MoeMatrix(_devptr(data), ld, stride, _devptr(scales), lds, stride_scales, _devptr(zeros), ldz, stride_zeros)
+    w.held = (data, scales, zeros)
+    return w
+
+
+def moe_layer(dtype, hidden, inner, experts, top_k, router, ld_router, gate_up, down, group=0, bias=None, scoring=MOE_SOFTMAX,
+              renormalize=True, router_dtype=None):
+    """A mixture-of-experts layer for moe(): gate_up and down from moe_matrix(), `group` of their 4-bit weights (0: weights of type dtype)."""
+    layer = MoeLayer(dtype, dtype if router_dtype is None else router_dtype, scoring, 1 if renormalize else 0, hidden, inner, experts, top_k, group,
+                     _devptr(router), ld_router, _devptr(bias), gate_up, down)
+    layer.held = (router, bias, gate_up, down)
+    return layer
+
+
+def moe_workspace_bytes(layer, tokens):
+    """Bytes of device memory that moe() needs for up to `tokens` tokens."""
+    n = lib().mmbo_moe_workspace_bytes(ctypes.byref(layer), tokens)
+    if n == 0:
+        _check(3)
+    return n
+
+
+def moe(layer, tokens, alpha, x, ldx, beta, y, ldy, workspace, workspace_bytes, ids=None, weights=None, stream=None):
+    """y = alpha * (the layer's output for `tokens` columns of x) + beta*y; asynchronous on `stream`.  ids (int32) and weights (float32) receive
+    the top_k experts of each token, best first.  Calls that may overlap in time need a workspace each."""
+    al, be = _scalars(F32, alpha, beta)
+    _check(lib().mmbo_moe(ctypes.byref(layer), tokens, ctypes.byref(al), _devptr(x), ldx, ctypes.byref(be), _devptr(y), ldy, _devptr(ids),
+                          _devptr(weights), _devptr(workspace), workspace_bytes, _stream_handle(stream)))
 
 
 def static_workspace_bytes():

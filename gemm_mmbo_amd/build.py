@@ -66,7 +66,7 @@ def _check_toolchain(verbose=True):
 
 
 def _units():
-    units = [("mmbo_gemm.hip", "mmbo_gemm.o", []), ("probe.hip", "probe.o", [])]
+    units = [("mmbo_gemm.hip", "mmbo_gemm.o", []), ("probe.hip", "probe.o", []), ("w4.hip", "w4.o", []), ("moe.hip", "moe.o", [])]
     for dtype in (0, 1):
         for tile in range(NUM_TILES):
             units.append(("inst_staged.hip", f"inst_staged_{dtype}_{tile}.o",

@@ -17,6 +17,7 @@
 #include "gemm_wave.hpp"
 #include "launch.hpp"
 #include "tuned_table.hpp"
+#include "w4.hpp"
 
 namespace mmbo {
 
@@ -441,6 +442,8 @@ double model_time_f64(int tile, size_t m, size_t n, size_t k, int batch)
 }
 
 }  // namespace
+
+int report_hip_error(hipError_t e) { return hip_fail(e); }
 
 hipError_t launch_splitk_reduce(int dtype, const GemmArgs &args, hipStream_t stream)
 {

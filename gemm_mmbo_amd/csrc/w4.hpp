@@ -1,0 +1,51 @@
+// Weights in 4 bits with a scale and a zero point for each group of k: the format, and what its kernels share.
+// (l, i): place l of k of row i.  Code (l, i) is half of byte (l + i * ldq) / 2, the low half for even l.
+#pragma once
+
+#include "gemm_common.hpp"
+
+namespace mmbo {
+
+typedef __bf16 bf16_t;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kW4Group = 32;               // groups are whole multiples of this
+constexpr float kW4Zero = 8.0f;                 // the zero point where none is stored
+
+// A weight as the kernels take it.
+struct W4Matrix {
+    const uint8_t *q;
+    const void *scales;
+    const uint8_t *zeros;                       // or null
+    uint64_t ldq;                               // bytes from row to row
+    uint64_t lds, ldz;                          // groups from row to row
+};
+
+struct GemmW4Args {
+    W4Matrix w;
+    const void *B;
+    void *C;
+    float alpha, beta;
+    uint32_t m, n, k, group;
+    uint64_t ldb, ldc;
+};
+
+struct QuantArgs {
+    W4Matrix w;                                 // (written by quantize)
+    void *W;                                    // (written by dequantize)
+    uint64_t ldw;
+    uint32_t m, k, group, groups;
+};
+
+inline bool w4_dtype(int dtype) { return dtype == 1 || dtype == 3; }             // MMBO_F16, MMBO_BF16
+
+template <typename Args, typename Kernel>
+inline hipError_t launch_args(Kernel kernel, dim3 grid, dim3 block, unsigned lds_bytes, hipStream_t stream, const Args &args)
+{
+    void *kargs[] = {const_cast<Args *>(&args)};
+    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, kargs, lds_bytes, stream);
+}
+
+int report_hip_error(hipError_t e);             // mmbo_gemm.hip: keeps the code for mmbo_last_hip_error
+
+}  // namespace mmbo

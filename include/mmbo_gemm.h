@@ -61,6 +61,7 @@ extern "C" {
 #define MMBO_F32 0
 #define MMBO_F16 1
 #define MMBO_F64 2
+#define MMBO_BF16 3             /* bfloat16: only the calls that name it take it (4-bit weights, mixture of experts) */
 
 #define MMBO_OP_N 0
 #define MMBO_OP_T 1
@@ -175,6 +176,100 @@ int mmbo_gemm_strided_batched_static_workspace(int dtype, int transA, int transB
                                                const void *beta, void *C, size_t ldc, long long strideC,
                                                int batch, int config_id, void *stream);
 size_t mmbo_static_workspace_bytes(void);
+
+/* ---- Products with 4-bit weights.  They have no counterpart in the reference (fp64 only); they are its product for the other
+ * end of the range, a few columns against a large weight that is read once and whose bytes are the time.
+ *
+ * The format: a weight W of m rows and k columns, stored row by row (k contiguous: op(A) of a product with transA = T), each
+ * element a code of 0 .. 15.  Code (l, i) -- place l of row i -- is half of byte (l + i*ldq) / 2 of Q: the low half for even l, the high
+ * half for odd.  ldq counts codes and is even (a row starts on a byte; no other alignment is asked for).  `group` consecutive places of a
+ * row share a scale and a zero point: group g = l / group, group a multiple of 32 (k need not be one, and group may exceed k);
+ * scales[g + i*lds] of type dtype, zeros[g + i*ldz] a byte.
+ *         W(l, i) = (code - zero) * scale;   zeros == NULL: every zero point is 8.
+ * dtype: MMBO_F16 or MMBO_BF16, of the scales and of everything the weights are multiplied with.  All launches are asynchronous on
+ * `stream`, allocate nothing and keep nothing: they can be captured, and calls on several streams share nothing.
+ * Dimensions and leading dimensions are at most 2^31 - 1. */
+
+/* C = alpha * W * B + beta * C: C(i, j) = alpha * sum_l W(l, i) * B[l + j*ldb] + beta * C[i + j*ldc], i < m, j < n, l < k; B and C of type
+ * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  The products are summed in fp32, a group's sum is
+ * multiplied by its scale in fp32, and one rounding to dtype follows at the store.  Any n: one column (a token of a
+ * decoding step) to thousands (a prompt).  The sum's order hangs on sizes, types and n alone: the same call gives the same bits.
+ * An infinity or a NaN in a column of B makes that column's results infinite or NaN; it reaches no other column. */
+int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const void *alpha, const void *Q, size_t ldq,
+                 const void *scales, size_t lds, const unsigned char *zeros, size_t ldz, const void *B, size_t ldb,
+                 const void *beta, void *C, size_t ldc, void *stream);
+
+/* W to that format, by rounding to nearest (halves to even): W[l + i*ldw] of type w_dtype (MMBO_F32, MMBO_F16, MMBO_BF16), scales of
+ * type dtype.  With zeros == NULL a group's scale is max|w| / 7 and its code round(w / scale) + 8; otherwise the scale is
+ * (max(w, 0) - min(w, 0)) / 15, the zero point round(-min(w, 0) / scale) and the code round(w / scale) + zero point, each within
+ * 0 .. 15.  The scale is rounded to fp32, then to dtype (at most its largest finite number), before it divides: codes fit the scale that is stored.
+ * A group whose scale is 0 gets codes equal to its zero point.  NaN counts as 0, an infinity as the largest finite
+ * number of w_dtype.  Codes behind k in a row's last byte are 0; other bytes of Q, scales and zeros are not touched. */
+int mmbo_w4_quantize(int w_dtype, int dtype, size_t m, size_t k, size_t group, const void *W, size_t ldw, void *Q, size_t ldq,
+                     void *scales, size_t lds, unsigned char *zeros, size_t ldz, void *stream);
+
+/* And back: W[l + i*ldw] = (code - zero) * scale in type dtype, one rounding. */
+int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *Q, size_t ldq, const void *scales, size_t lds,
+                       const unsigned char *zeros, size_t ldz, void *W, size_t ldw, void *stream);
+
+/* ---- A mixture-of-experts layer for a few tokens: router, selection, the chosen experts' products and their sum.  No counterpart in
+ * the reference; it is its strided batch (src/gemm/gemm.h:61-69) where the data says which problems of the batch each column
+ * takes part in.
+ *
+ *   logit(e, t) = sum_l router[l + e*ld_router] * x[l + t*ldx], summed in 64 bits: what is selected does not hang on the sum's order
+ *   score = softmax of a token's logits over the experts (MMBO_MOE_SOFTMAX) or 1 / (1 + exp(-logit)) (MMBO_MOE_SIGMOID)
+ *   selected: the top_k experts with the largest logit -- with a bias: the largest score + bias[e] --, ties to the lower index,
+ *       NaN behind everything else
+ *   weight = score, or (renormalize) score over the sum of the selected scores; 0 where that sum is 0
+ *   h = silu(gate * x) * (up * x), silu(v) = v / (1 + exp(-v));  y = alpha * sum over the selected of weight * (down * h) + beta * y
+ *
+ * Expert e's gate and up are rows 0 .. inner-1 and inner .. 2*inner-1 of one matrix of 2*inner rows and `hidden` columns, gate_up;
+ * down has `hidden` rows and `inner` columns; both row by row (k contiguous).  group == 0: elements of type dtype, data[l + i*ld +
+ * e*stride]; otherwise 4-bit weights in the format above with that group: code (l, i) of expert e is code number l + i*ld + e*stride (both even),
+ * its scale scales[g + i*lds + e*stride_scales], its zero point zeros[g + i*ldz + e*stride_zeros] (zeros NULL: 8).
+ * h is held as the sum of two numbers of type dtype (an h beyond that type's range is infinite), every sum in fp32. */
+#define MMBO_MOE_SOFTMAX 0
+#define MMBO_MOE_SIGMOID 1
+#define MMBO_MOE_MAX_TOKENS 512
+#define MMBO_MOE_MAX_EXPERTS 512
+#define MMBO_MOE_MAX_TOP_K 32
+
+typedef struct mmbo_moe_matrix {
+    const void *data;
+    size_t ld;
+    long long stride;
+    const void *scales;             /* the rest for 4-bit weights only */
+    size_t lds;
+    long long stride_scales;
+    const unsigned char *zeros;
+    size_t ldz;
+    long long stride_zeros;
+} mmbo_moe_matrix;
+
+typedef struct mmbo_moe_layer {
+    int dtype;                      /* MMBO_F16 or MMBO_BF16: of x, y and the weights (4-bit ones: of their scales) */
+    int router_dtype;               /* dtype or MMBO_F32 */
+    int scoring;
+    int renormalize;
+    size_t hidden, inner, experts, top_k;
+    size_t group;                   /* of 4-bit weights; 0: weights of type dtype */
+    const void *router;
+    size_t ld_router;
+    const float *bias;              /* per expert, or NULL */
+    mmbo_moe_matrix gate_up, down;
+} mmbo_moe_layer;
+
+/* Bytes of device memory (16-byte aligned) that a call with up to `tokens` tokens needs as a workspace; 0 on bad arguments.  Pure
+ * host logic. */
+size_t mmbo_moe_workspace_bytes(const mmbo_moe_layer *layer, size_t tokens);
+
+/* x: hidden x tokens, y: hidden x tokens, column after column; ids and weights (either may be NULL) receive the selection, best first:
+ * ids[s + t*top_k], weights[s + t*top_k].  The layer is read before the call returns, device memory it points to by the launches,
+ * which are asynchronous on `stream`.  The workspace is the caller's: no contents are expected or left behind, it may serve
+ * one call after another on one stream, but calls (or graphs) that may overlap in time need one each; too small a one is refused
+ * with MMBO_ERR_WORKSPACE.  Nothing is allocated: the call can be captured.  Same call, same bits. */
+int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, const void *x, size_t ldx, const void *beta, void *y,
+             size_t ldy, int *ids, float *weights, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Release the split-K workspaces held for the current device (one per stream that ran a split-K config; allocated
  * lazily, grown on demand, reused across calls).  Waits for the device.  The reference never frees what it loads
