@@ -57,4 +57,7 @@ hipError_t launch_dots(int transA, int transB, const GemmArgs &args, hipStream_t
 
 hipError_t launch_splitk_reduce(int dtype, const GemmArgs &args, hipStream_t stream);
 
+// Keeps the code for mmbo_last_hip_error; returns MMBO_ERR_HIP.
+int report_hip_error(hipError_t e);
+
 }  // namespace mmbo

@@ -17,7 +17,6 @@
 #include "gemm_wave.hpp"
 #include "launch.hpp"
 #include "tuned_table.hpp"
-#include "w4.hpp"
 
 namespace mmbo {
 

@@ -36,7 +36,7 @@ __device__ inline float weight(const MoeMatrix &m, uint32_t expert, uint64_t i, 
     if constexpr (!W4) return (float)reinterpret_cast<const T *>(q)[l];
     const uint32_t g = l / group;
     const float s = (float)static_cast<const T *>(m.w4.scales)[(int64_t)expert * m.stride_scales + g + i * m.w4.lds];
-    const float z = m.w4.zeros ? (float)m.w4.zeros[(int64_t)expert * m.stride_zeros + g + i * m.w4.ldz] : kW4Zero;
+    const float z = m.w4.zeros ? (float)(m.w4.zeros[(int64_t)expert * m.stride_zeros + g + i * m.w4.ldz] & kW4ZeroMask) : kW4Zero;
     return ((float)(l & 1 ? q[l / 2] >> 4 : q[l / 2] & 15) - z) * s;
 }
 

@@ -2,48 +2,16 @@
 #include "../../include/mmbo_gemm.h"
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
-#include "w4.hpp"
+#include "w4_stream.hpp"
 
 namespace mmbo {
 namespace {
 
 template <typename T>
 __device__ inline float load_scale(const void *p, uint64_t at) { return (float)static_cast<const T *>(p)[at]; }
-
-// A wavefront has one row of W and up to four columns of B; its lanes share k, eight places of a dword of codes at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_w4_rows_kernel(const GemmW4Args a)
-{
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t i = (uint64_t)blockIdx.x * 4 + wave;
-    if (i >= a.m) return;
-    for (uint64_t j0 = (uint64_t)blockIdx.y * 4; j0 < a.n; j0 += (uint64_t)gridDim.y * 4) {
-        float acc[4] = {};
-        for (uint64_t l0 = lane * 8; l0 < a.k; l0 += 512) {
-            const uint32_t g = (uint32_t)(l0 / a.group);
-            const float s = load_scale<T>(a.w.scales, g + i * a.w.lds);
-            const float z = a.w.zeros ? (float)a.w.zeros[g + i * a.w.ldz] : kW4Zero;
-            for (uint32_t e = 0; e < 8 && l0 + e < a.k; ++e) {
-                const uint64_t l = l0 + e;
-                const uint8_t byte = a.w.q[i * a.w.ldq + l / 2];
-                const float w = ((float)(l & 1 ? byte >> 4 : byte & 15) - z) * s;
-                for (uint32_t j = 0; j < 4; ++j)
-                    if (j0 + j < a.n) acc[j] = __builtin_fmaf(w, (float)static_cast<const T *>(a.B)[l + (j0 + j) * a.ldb], acc[j]);
-            }
-        }
-        for (uint32_t j = 0; j < 4; ++j) {
-            float v = acc[j];
-            for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-            if (lane == 0 && j0 + j < a.n) {
-                T *c = static_cast<T *>(a.C) + i + (j0 + j) * a.ldc;
-                v *= a.alpha;
-                if (a.beta != 0.0f) v = __builtin_fmaf(a.beta, (float)*c, v);
-                *c = (T)v;
-            }
-        }
-    }
-}
 
 template <typename T> struct Limits;
 template <> struct Limits<float> { static constexpr float largest = 3.40282346638528859812e38f; };
@@ -111,7 +79,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
     const uint64_t i = at / a.k, l = at % a.k;
     const uint32_t g = (uint32_t)(l / a.group);
     const uint8_t byte = a.w.q[i * a.w.ldq + l / 2];
-    const float z = a.w.zeros ? (float)a.w.zeros[g + i * a.w.ldz] : kW4Zero;
+    const float z = a.w.zeros ? (float)(a.w.zeros[g + i * a.w.ldz] & kW4ZeroMask) : kW4Zero;
     static_cast<T *>(a.W)[i * a.ldw + l] = (T)(((float)(l & 1 ? byte >> 4 : byte & 15) - z) * load_scale<T>(a.w.scales, g + i * a.w.lds));
 }
 
@@ -135,6 +103,72 @@ W4Matrix matrix_of(const void *Q, size_t ldq, const void *scales, size_t lds, co
 
 int status_of(hipError_t e) { return e == hipSuccess ? MMBO_OK : report_hip_error(e); }
 
+template <typename Kernel>
+hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire))) return e;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == hipSuccess && dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+    return e;
+}
+
+constexpr int kStreamWaves = 8;
+
+template <typename T, int N2, int FT, int FOLDS>
+hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
+{
+    // Blocks under way in a ring.  Work-groups beside each other on a CU hide what a deeper ring would, and need the LDS: 28672 x 1 x 8192 29.4 us
+    // with rings of 3, 28.4 of 2, 33.7 of 3 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 of 2, 13.6 of 3, 14.5 of 4.
+    constexpr int DEPTH = N2 == 1 ? 3 : 2;
+    typedef stream::Stream4<T, N2, FT, FOLDS, DEPTH> S;
+    static_assert(kStreamWaves * S::LDS_BYTES <= 160 * 1024, "a work-group's rings do not fit the 160 KB of LDS");
+    static std::atomic<bool> set[64];
+    auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLDS, DEPTH>;
+    if (hipError_t e = allow_lds(kernel, set)) return e;
+    int waves = 1;
+    while (waves < kStreamWaves && (uint32_t)waves * S::BLOCK < a.k) waves *= 2;
+    return launch_args(kernel, dim3((unsigned)ceil_div(a.m, 16 * FT)), dim3(waves * 64), waves * S::LDS_BYTES, s, a);
+}
+
+template <typename T, int N2, int FT>
+hipError_t launch_stream_tile(const GemmW4Args &a, hipStream_t s)
+{
+    if (a.group % 128 == 0) return launch_stream_kernel<T, N2, FT, 1>(a, s);
+    if (a.group % 64 == 0) return launch_stream_kernel<T, N2, FT, 2>(a, s);
+    return launch_stream_kernel<T, N2, FT, 4>(a, s);
+}
+
+template <typename T, int N2>
+hipError_t launch_stream_columns(const GemmW4Args &a, hipStream_t s)
+{
+    // Two tiles of rows a work-group where that still is a work-group for each of 256 CUs: the columns, which every work-group reads, are then read half as
+    // often.  8192 x 16 x 8192 11.3 us beside 14.5, 128256 x 1 x 4096 53.9 beside 61.3; 4096 x 16 x 14336 16.2 beside 13.3.
+    return a.m >= 256 * 32 ? launch_stream_tile<T, N2, 2>(a, s) : launch_stream_tile<T, N2, 1>(a, s);
+}
+
+template <typename T>
+hipError_t launch_stream(const GemmW4Args &all, hipStream_t s)
+{
+    constexpr uint32_t kRows = 1u << 26;         // of one launch: a grid has less than 2^32 threads
+    for (uint64_t i = 0; i < all.m; i += kRows)
+        for (uint64_t j = 0; j < all.n; j += 16) {
+            GemmW4Args a = all;
+            a.m = (uint32_t)std::min<uint64_t>(all.m - i, kRows);
+            a.n = (uint32_t)std::min<uint64_t>(all.n - j, 16);
+            a.w.q += i * a.w.ldq;
+            a.w.scales = static_cast<const T *>(a.w.scales) + i * a.w.lds;
+            if (a.w.zeros) a.w.zeros += i * a.w.ldz;
+            a.B = static_cast<const T *>(all.B) + j * all.ldb;
+            a.C = static_cast<T *>(all.C) + i + j * all.ldc;
+            const hipError_t e = a.n == 1 ? launch_stream_columns<T, 1>(a, s) : a.n <= 4 ? launch_stream_columns<T, 4>(a, s)
+                               : a.n <= 8 ? launch_stream_columns<T, 8>(a, s) : launch_stream_columns<T, 16>(a, s);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+
 }  // namespace
 }  // namespace mmbo
 
@@ -155,10 +189,8 @@ int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const vo
     if (!C || (k != 0 && (!Q || !scales || !B))) return MMBO_ERR_NULL_POINTER;
     const GemmW4Args a{matrix_of(Q, ldq, scales, lds, zeros, ldz), B, C, *static_cast<const float *>(alpha), *static_cast<const float *>(beta),
                        (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)group, ldb, ldc};
-    const dim3 grid((unsigned)((m + 3) / 4), (unsigned)std::min<size_t>((n + 3) / 4, 65535));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return status_of(dtype == MMBO_F16 ? launch_args(gemm_w4_rows_kernel<half_t>, grid, dim3(256), 0, s, a)
-                                       : launch_args(gemm_w4_rows_kernel<bf16_t>, grid, dim3(256), 0, s, a));
+    return status_of(dtype == MMBO_F16 ? launch_stream<half_t>(a, s) : launch_stream<bf16_t>(a, s));
 }
 
 int mmbo_w4_quantize(int w_dtype, int dtype, size_t m, size_t k, size_t group, const void *W, size_t ldw, void *Q, size_t ldq,

@@ -2,7 +2,7 @@
 // (l, i): place l of k of row i.  Code (l, i) is half of byte (l + i * ldq) / 2, the low half for even l.
 #pragma once
 
-#include "gemm_common.hpp"
+#include "launch.hpp"
 
 namespace mmbo {
 
@@ -11,6 +11,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kW4Group = 32;               // groups are whole multiples of this
 constexpr float kW4Zero = 8.0f;                 // the zero point where none is stored
+constexpr uint8_t kW4ZeroMask = 127;            // what counts of a stored one: 128 + zero point has to be a bf16 number
 
 // A weight as the kernels take it.
 struct W4Matrix {
@@ -37,6 +38,9 @@ struct QuantArgs {
     uint32_t m, k, group, groups;
 };
 
+template <typename N>
+constexpr size_t ceil_div(size_t n, N by) { return (n + by - 1) / by; }
+
 inline bool w4_dtype(int dtype) { return dtype == 1 || dtype == 3; }             // MMBO_F16, MMBO_BF16
 
 template <typename Args, typename Kernel>
@@ -45,7 +49,5 @@ inline hipError_t launch_args(Kernel kernel, dim3 grid, dim3 block, unsigned lds
     void *kargs[] = {const_cast<Args *>(&args)};
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, kargs, lds_bytes, stream);
 }
-
-int report_hip_error(hipError_t e);             // mmbo_gemm.hip: keeps the code for mmbo_last_hip_error
 
 }  // namespace mmbo

@@ -184,7 +184,7 @@ size_t mmbo_static_workspace_bytes(void);
  * element a code of 0 .. 15.  Code (l, i) -- place l of row i -- is half of byte (l + i*ldq) / 2 of Q: the low half for even l, the high
  * half for odd.  ldq counts codes and is even (a row starts on a byte; no other alignment is asked for).  `group` consecutive places of a
  * row share a scale and a zero point: group g = l / group, group a multiple of 32 (k need not be one, and group may exceed k);
- * scales[g + i*lds] of type dtype, zeros[g + i*ldz] a byte.
+ * scales[g + i*lds] of type dtype, zeros[g + i*ldz] a byte, of which the low seven bits count.
  *         W(l, i) = (code - zero) * scale;   zeros == NULL: every zero point is 8.
  * dtype: MMBO_F16 or MMBO_BF16, of the scales and of everything the weights are multiplied with.  All launches are asynchronous on
  * `stream`, allocate nothing and keep nothing: they can be captured, and calls on several streams share nothing.
@@ -194,7 +194,8 @@ size_t mmbo_static_workspace_bytes(void);
  * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  The products are summed in fp32, a group's sum is
  * multiplied by its scale in fp32, and one rounding to dtype follows at the store.  Any n: one column (a token of a
  * decoding step) to thousands (a prompt).  The sum's order hangs on sizes, types and n alone: the same call gives the same bits.
- * An infinity or a NaN in a column of B makes that column's results infinite or NaN; it reaches no other column. */
+ * An infinity or a NaN in a column of B makes that column's results infinite or NaN (so do, in bf16, elements beyond 2^119); it
+ * reaches no other column. */
 int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const void *alpha, const void *Q, size_t ldq,
                  const void *scales, size_t lds, const unsigned char *zeros, size_t ldz, const void *B, size_t ldb,
                  const void *beta, void *C, size_t ldc, void *stream);
