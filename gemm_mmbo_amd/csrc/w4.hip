@@ -5,7 +5,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "w4_stream.hpp"
+#include "stream.hpp"
 
 namespace mmbo {
 namespace {
@@ -116,28 +116,34 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
 
 constexpr int kStreamWaves = 8;
 
-template <typename T, int N2, int FT, int FOLDS>
+template <typename T, int N2, int FT, int FOLDS, bool ZEROS>
 hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
 {
     // Blocks under way in a ring.  Work-groups beside each other on a CU hide what a deeper ring would, and need the LDS: 28672 x 1 x 8192 29.4 us
     // with rings of 3, 28.4 of 2, 33.7 of 3 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 of 2, 13.6 of 3, 14.5 of 4.
     constexpr int DEPTH = N2 == 1 ? 3 : 2;
-    typedef stream::Stream4<T, N2, FT, FOLDS, DEPTH> S;
-    static_assert(kStreamWaves * S::LDS_BYTES <= 160 * 1024, "a work-group's rings do not fit the 160 KB of LDS");
+    typedef stream::Stream<T, true, N2, FT, 1, FOLDS, ZEROS, DEPTH> S;
+    constexpr int kWaveBytes = std::max(S::LDS_BYTES, stream::tiles_of<N2>() * FT * 1024);
+    constexpr int kMost = std::min(kStreamWaves, 160 * 1024 / kWaveBytes);
     static std::atomic<bool> set[64];
-    auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLDS, DEPTH>;
+    auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLDS, ZEROS, DEPTH>;
     if (hipError_t e = allow_lds(kernel, set)) return e;
-    int waves = 1;
-    while (waves < kStreamWaves && (uint32_t)waves * S::BLOCK < a.k) waves *= 2;
-    return launch_args(kernel, dim3((unsigned)ceil_div(a.m, 16 * FT)), dim3(waves * 64), waves * S::LDS_BYTES, s, a);
+    const int waves = (int)std::max<uint32_t>(std::min<uint32_t>(S::blocks_of(a.k), kMost), 1);
+    return launch_args(kernel, dim3((unsigned)ceil_div(a.m, 16 * FT)), dim3(waves * 64), waves * kWaveBytes, s, a);
+}
+
+template <typename T, int N2, int FT, int FOLDS>
+hipError_t launch_stream_folds(const GemmW4Args &a, hipStream_t s)
+{
+    return a.w.zeros ? launch_stream_kernel<T, N2, FT, FOLDS, true>(a, s) : launch_stream_kernel<T, N2, FT, FOLDS, false>(a, s);
 }
 
 template <typename T, int N2, int FT>
 hipError_t launch_stream_tile(const GemmW4Args &a, hipStream_t s)
 {
-    if (a.group % 128 == 0) return launch_stream_kernel<T, N2, FT, 1>(a, s);
-    if (a.group % 64 == 0) return launch_stream_kernel<T, N2, FT, 2>(a, s);
-    return launch_stream_kernel<T, N2, FT, 4>(a, s);
+    if (a.group % 128 == 0) return launch_stream_folds<T, N2, FT, 1>(a, s);
+    if (a.group % 64 == 0) return launch_stream_folds<T, N2, FT, 2>(a, s);
+    return launch_stream_folds<T, N2, FT, 4>(a, s);
 }
 
 template <typename T, int N2>
@@ -153,17 +159,17 @@ hipError_t launch_stream(const GemmW4Args &all, hipStream_t s)
 {
     constexpr uint32_t kRows = 1u << 26;         // of one launch: a grid has less than 2^32 threads
     for (uint64_t i = 0; i < all.m; i += kRows)
-        for (uint64_t j = 0; j < all.n; j += 16) {
+        for (uint64_t j = 0; j < all.n; j += 32) {
             GemmW4Args a = all;
             a.m = (uint32_t)std::min<uint64_t>(all.m - i, kRows);
-            a.n = (uint32_t)std::min<uint64_t>(all.n - j, 16);
+            a.n = (uint32_t)std::min<uint64_t>(all.n - j, 32);
             a.w.q += i * a.w.ldq;
             a.w.scales = static_cast<const T *>(a.w.scales) + i * a.w.lds;
             if (a.w.zeros) a.w.zeros += i * a.w.ldz;
             a.B = static_cast<const T *>(all.B) + j * all.ldb;
             a.C = static_cast<T *>(all.C) + i + j * all.ldc;
             const hipError_t e = a.n == 1 ? launch_stream_columns<T, 1>(a, s) : a.n <= 4 ? launch_stream_columns<T, 4>(a, s)
-                               : a.n <= 8 ? launch_stream_columns<T, 8>(a, s) : launch_stream_columns<T, 16>(a, s);
+                               : a.n <= 16 ? launch_stream_columns<T, 16>(a, s) : launch_stream_columns<T, 32>(a, s);
             if (e != hipSuccess) return e;
         }
     return hipSuccess;

@@ -234,6 +234,7 @@ int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *
 #define MMBO_MOE_MAX_TOKENS 512
 #define MMBO_MOE_MAX_EXPERTS 512
 #define MMBO_MOE_MAX_TOP_K 32
+#define MMBO_MOE_MAX_DIM 65536          /* hidden, inner */
 
 typedef struct mmbo_moe_matrix {
     const void *data;

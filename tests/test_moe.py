@@ -31,7 +31,7 @@ def _status(layer, tokens=2, x=16, ldx=64, y=16, ldy=64, workspace=16, nbytes=1 
 
 
 @pytest.mark.parametrize("layer,status", [
-    (dict(dtype=F32), 1), (dict(dtype=F64), 1), (dict(dtype=F16, router_dtype=BF16), 1), (dict(scoring=2), 2), (dict(hidden=0), 3), (dict(inner=0), 3),
+    (dict(dtype=F32), 1), (dict(dtype=F64), 1), (dict(dtype=F16, router_dtype=BF16), 1), (dict(scoring=2), 2), (dict(hidden=0), 3), (dict(inner=0), 3), (dict(hidden=65537, ld_router=65537), 3), (dict(inner=65537), 3),
     (dict(experts=0), 3), (dict(experts=G.MOE_MAX_EXPERTS + 1), 3), (dict(top_k=0), 3), (dict(top_k=5), 3), (dict(experts=64, top_k=G.MOE_MAX_TOP_K + 1), 3),
     (dict(group=16), 3), (dict(group=2 ** 31), 3), (dict(ld_router=63), 3), (dict(gate_up=G.moe_matrix(16, 63, 1 << 20)), 3), (dict(down=G.moe_matrix(16, 31, 1 << 20)), 3),
     (dict(down=G.moe_matrix(16, 32, -64)), 3), (dict(group=32, gate_up=G.moe_matrix(16, 64, 1 << 20, 16, 1)), 3), (dict(group=32, gate_up=G.moe_matrix(16, 65, 1 << 20, 16, 2)), 3),
