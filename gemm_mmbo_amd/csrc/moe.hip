@@ -10,6 +10,8 @@
 namespace mmbo {
 namespace {
 
+constexpr uint32_t kTokens = 64;                // worked on at a time: a row of the grids
+
 struct MoeMatrix {
     W4Matrix w4;                                // 4-bit weights; of 16-bit ones w4.q is their address and w4.ldq their bytes from row to row
     int64_t stride, stride_scales, stride_zeros;    // bytes, groups, groups from expert to expert
@@ -23,11 +25,16 @@ struct MoeArgs {
     double *logits;                             // [tokens][experts]
     void *h;                                    // [2][tokens * top_k][ld_h], of the layer's type
     char *table;                                // of each row of tokens
+    float *parts;                               // sums of work-groups that share a tile of y: [row of tokens][tile][sharer][token][element]
+    uint32_t *arrived;                          // how many of them are done: [row of tokens][tile]
+    uint32_t *chosen;                           // the selection: [tokens][top_k]
+    float *chosen_weights;
+    uint32_t *selected;                         // work-groups of a row that have selected
     int *ids;                                   // [tokens][top_k]; either may be null
     float *weights;
     float alpha, beta;
     uint32_t tokens, hidden, inner, experts, top_k, group;
-    uint32_t ld_h, columns, most_jobs;
+    uint32_t ld_h, columns, most_jobs, down_tiles, sharers;
     uint64_t ldx, ldy, ld_router;
     int sigmoid, renormalize;
 };
@@ -60,6 +67,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a)
 {
     __shared__ double parts[4][kLogitTokens];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x, t0 = blockIdx.y * kLogitTokens;
+    if (e == 0 && t0 % kTokens == 0 && threadIdx.x == 0) a.selected[t0 / kTokens] = 0;
     const uint32_t count = min(kLogitTokens, a.tokens - t0);
     const TR *r = static_cast<const TR *>(a.router) + e * a.ld_router;
     const T *x = static_cast<const T *>(a.x) + t0 * a.ldx;
@@ -84,8 +92,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a)
         a.logits[(uint64_t)(t0 + threadIdx.x) * a.experts + e] = parts[0][threadIdx.x] + parts[1][threadIdx.x] + parts[2][threadIdx.x] + parts[3][threadIdx.x];
 }
 
-// Up to kTokens tokens are worked on at a time (a row of the grids).  Their (token, slot) pairs by expert, and each expert's pairs in jobs of up to `columns`.
-constexpr uint32_t kTokens = 64;
+// The (token, slot) pairs of a row of tokens by expert, and each expert's pairs in jobs of up to `columns`.
 struct Table {
     uint32_t *count;                            // of jobs
     float *weight;                              // of a pair
@@ -131,134 +138,232 @@ __device__ inline uint64_t wave_max(uint64_t v)
     return max((uint64_t)h32[0] << 32 | l32[0], (uint64_t)h32[1] << 32 | l32[1]);
 }
 
-// A work-group: the selection of a row's tokens, a wavefront a token at a time, and the row's table.  PER: experts a lane has, lane + 64 * b.
+// The selection of one token by a wavefront: lane s gets the expert of slot s and its weight.  PER: experts a lane has, lane + 64 * b.
 template <int PER>
-__global__ void __launch_bounds__(1024) moe_select_kernel(const MoeArgs a)
+__device__ inline void select_token(const MoeArgs &a, uint32_t token, uint32_t lane, uint32_t &expert, float &weight)
 {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint32_t token0 = blockIdx.x * kTokens, tokens = min(kTokens, a.tokens - token0), pairs = tokens * a.top_k, most_pairs = min(kTokens, a.tokens) * a.top_k;
-    float *const weight = reinterpret_cast<float *>(lds);                               // by token and slot
-    uint16_t *const id = reinterpret_cast<uint16_t *>(weight + most_pairs), *const before = id + most_pairs, *const jobs_before = before + a.experts;
-    for (uint32_t t = wave; t < tokens; t += waves) {
-        const double *logits = a.logits + (uint64_t)(token0 + t) * a.experts;
-        double logit[PER];
-        uint64_t key[PER];
-        uint64_t most = 0;
+    const double *logits = a.logits + (uint64_t)token * a.experts;
+    double logit[PER];
+    uint64_t key[PER];
+    uint64_t most = 0;
 #pragma unroll
-        for (int b = 0; b < PER; ++b) {
-            const uint32_t e = lane + 64 * b;
-            logit[b] = e < a.experts ? logits[e] : -__builtin_huge_val();
-            key[b] = e < a.experts ? order_of(logit[b]) : 0;
-            most = max(most, key[b]);
-        }
-        double sum = 0.0, highest = 0.0;
-        if (!a.sigmoid) {
-            // (a NaN among the logits is no largest one; it makes the sum NaN, which scores that only count against each other do not need)
-            most = wave_max(most);
-            highest = __builtin_bit_cast(double, most >> 63 ? most & ~(1ull << 63) : ~most);
-            if (!a.renormalize || a.bias) {
+    for (int b = 0; b < PER; ++b) {
+        const uint32_t e = lane + 64 * b;
+        logit[b] = e < a.experts ? logits[e] : -__builtin_huge_val();
+        key[b] = e < a.experts ? order_of(logit[b]) : 0;
+        most = max(most, key[b]);
+    }
+    // (One exp for all cases: on a CU that runs this once, time goes into fetching instructions.  A NaN among the logits is no largest one; it makes the
+    // sum NaN, which scores that only count against each other do not need.)
+    const bool over_sum = !a.sigmoid && (!a.renormalize || a.bias);
+    if (!a.sigmoid) most = wave_max(most);
+    const double highest = __builtin_bit_cast(double, most >> 63 ? most & ~(1ull << 63) : ~most);
+    double score[PER], sum = 0.0;
 #pragma unroll
-                for (int b = 0; b < PER; ++b)
-                    if (lane + 64 * b < a.experts) sum += exp(logit[b] - highest);
-                sum = wave_sum(sum);
-            }
-        }
-        // (not over its sum where only selected scores count against each other)
-        auto score = [&](double v) { return a.sigmoid ? 1.0 / (1.0 + exp(-v)) : !a.renormalize || a.bias ? exp(v - highest) / sum : exp(v - highest); };
-        if (a.bias)
+    for (int b = 0; b < PER; ++b) {
+        const double v = exp(a.sigmoid ? -logit[b] : logit[b] - highest);
+        score[b] = a.sigmoid ? 1.0 / (1.0 + v) : v;
+        if (lane + 64 * b < a.experts) sum += v;
+    }
+    if (over_sum) {
+        sum = 1.0 / wave_sum(sum);
 #pragma unroll
-            for (int b = 0; b < PER; ++b)
-                if (lane + 64 * b < a.experts) key[b] = order_of(score(logit[b]) + (double)a.bias[lane + 64 * b]);
-        uint32_t mine = 0, here = 0;             // the expert of slot `lane`; of this lane's experts, those that may still be taken
+        for (int b = 0; b < PER; ++b) score[b] *= sum;
+    }
+    if (a.bias)
 #pragma unroll
         for (int b = 0; b < PER; ++b)
-            if (lane + 64 * b < a.experts) here |= 1u << b;
-        for (uint32_t s = 0; s < a.top_k; ++s) {
-            uint64_t best = 0;
+            if (lane + 64 * b < a.experts) key[b] = order_of(score[b] + (double)a.bias[lane + 64 * b]);
+    uint32_t mine = 0, here = 0;             // the expert of slot `lane`; of this lane's experts, those that may still be taken
+    double mine_score = 0.0;
 #pragma unroll
-            for (int b = 0; b < PER; ++b)
-                if (here >> b & 1) best = max(best, key[b]);
-            best = wave_max(best);
-            uint32_t e = 0;
-            bool found = false;
+    for (int b = 0; b < PER; ++b)
+        if (lane + 64 * b < a.experts) here |= 1u << b;
+    for (uint32_t s = 0; s < a.top_k; ++s) {
+        uint64_t best = 0;
 #pragma unroll
-            for (int b = 0; b < PER; ++b) {
-                const uint64_t who = __ballot((here >> b & 1) && key[b] == best);
-                if (!found && who != 0) {
-                    e = 64 * b + __builtin_ctzll(who);
-                    found = true;
-                }
+        for (int b = 0; b < PER; ++b)
+            if (here >> b & 1) best = max(best, key[b]);
+        best = wave_max(best);
+        uint32_t e = 0;
+        double v = 0.0;
+        bool found = false;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) {
+            const uint64_t who = __ballot((here >> b & 1) && key[b] == best);
+            if (!found && who != 0) {
+                const int l = __builtin_ctzll(who);
+                const uint64_t bits = __builtin_bit_cast(uint64_t, score[b]);
+                e = 64 * b + l;
+                v = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(bits >> 32), l) << 32 |
+                                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)bits, l));
+                found = true;
             }
-            if (lane == (e & 63)) here &= ~(1u << (e >> 6));
-            if (lane == s) mine = e;
         }
-        double v = lane < a.top_k ? score(logits[mine]) : 0.0;
-        if (a.renormalize) {
-            const double total = wave_sum(v);
-            v = total == 0.0 ? 0.0 : v / total;
-        }
-        if (lane < a.top_k) {
-            const uint32_t p = t * a.top_k + lane;
-            id[p] = (uint16_t)mine;
-            weight[p] = (float)v;
-            if (a.ids) a.ids[(uint64_t)token0 * a.top_k + p] = (int)mine;
-            if (a.weights) a.weights[(uint64_t)token0 * a.top_k + p] = (float)v;
+        if (lane == (e & 63)) here &= ~(1u << (e >> 6));
+        if (lane == s) {
+            mine = e;
+            mine_score = v;
         }
     }
+    double v = mine_score;
+    if (a.renormalize) {
+        const double total = wave_sum(v);
+        v = total == 0.0 ? 0.0 : v / total;
+    }
+    expert = mine;
+    weight = (float)v;
+}
+__device__ inline void select_token(const MoeArgs &a, uint32_t token, uint32_t lane, uint32_t &expert, float &weight)
+{
+    if (a.experts <= 64) select_token<1>(a, token, lane, expert, weight);
+    else if (a.experts <= 128) select_token<2>(a, token, lane, expert, weight);
+    else select_token<8>(a, token, lane, expert, weight);
+}
+
+// A row's selection in LDS, and what a work-group needs to make its table.
+struct Selection {
+    uint16_t *id;                               // of a pair; whole eights of them
+    float *weight;
+    uint16_t *pair;                             // pairs by expert
+    uint16_t *before;                           // of a part of the pairs, for an expert: pairs by expert in front of it
+    uint16_t *jobs_before;                      // of an expert
+};
+constexpr uint32_t kMostParts = 512;            // (no work-group has more threads)
+__host__ __device__ inline uint32_t select_bytes(uint32_t pairs, uint32_t experts)
+{
+    return ((pairs + 7) / 8 * 16 + pairs * 4 + (pairs + kMostParts + 2 * experts) * 2 + 15) / 16 * 16;
+}
+__device__ inline Selection selection_at(char *lds, uint32_t most_pairs, uint32_t experts)
+{
+    Selection s;
+    s.id = reinterpret_cast<uint16_t *>(lds);
+    s.weight = reinterpret_cast<float *>(s.id + (most_pairs + 7) / 8 * 8);
+    s.pair = reinterpret_cast<uint16_t *>(s.weight + most_pairs);
+    s.jobs_before = s.pair + most_pairs;
+    s.before = s.jobs_before + experts;
+    return s;
+}
+
+// Sums of those in front of each of n numbers (their sum stays below 2^16), by one wavefront; their sum.
+__device__ inline uint32_t scan(uint16_t *v, uint32_t n, uint32_t lane)
+{
+    uint32_t total = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const uint32_t own = i0 + lane < n ? v[i0 + lane] : 0;
+        uint32_t sum = own;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t other = __shfl_up(sum, d);
+            if ((int)lane >= d) sum += other;
+        }
+        if (i0 + lane < n) v[i0 + lane] = (uint16_t)(total + sum - own);
+        total += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return total;
+}
+
+// The table of `pairs` pairs, by a work-group that has them in LDS.  A thread looks through a part of the pairs for an expert's, eight ids at a time: one thread
+// to an expert, and a store to memory a pair, was 12 us for 128 pairs.
+__device__ inline void make_table(const MoeArgs &a, uint32_t pairs, const Selection &sel, const Table &table)
+{
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 *const id8 = reinterpret_cast<const u16x8 *>(sel.id);
+    const uint32_t eights = (pairs + 7) / 8, parts = max(min(blockDim.x / a.experts, eights), 1u);
+    if (threadIdx.x < eights * 8 - pairs) sel.id[pairs + threadIdx.x] = 0xFFFF;
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) {
+    for (uint32_t x = threadIdx.x; x < a.experts * parts; x += blockDim.x) {
+        const uint32_t e = x / parts, part = x % parts;
         uint32_t n = 0;
-        for (uint32_t p = 0; p < pairs; ++p) n += id[p] == e;
-        before[e] = (uint16_t)n;
-        jobs_before[e] = (uint16_t)((n + a.columns - 1) / a.columns);
+        for (uint32_t q = eights * part / parts; q < eights * (part + 1) / parts; ++q) {
+            const u16x8 v = id8[q];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n += v[i] == e;
+        }
+        sel.before[x] = (uint16_t)n;
     }
     __syncthreads();
-    const Table table = table_at(a.table + (uint64_t)blockIdx.x * table_bytes(most_pairs, a.most_jobs), most_pairs, a.most_jobs);
-    if (threadIdx.x < 64) {                      // sums of those in front
-        uint32_t n0 = 0, j0 = 0;
-        for (uint32_t e0 = 0; e0 < a.experts; e0 += 64) {
-            const uint32_t e = e0 + threadIdx.x;
-            const uint32_t n = e < a.experts ? before[e] : 0, j = e < a.experts ? jobs_before[e] : 0;
-            uint32_t ns = n, js = j;
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t nn = __shfl_up(ns, d), jj = __shfl_up(js, d);
-                if ((int)threadIdx.x >= d) { ns += nn; js += jj; }
-            }
-            if (e < a.experts) {
-                before[e] = (uint16_t)(n0 + ns - n);
-                jobs_before[e] = (uint16_t)(j0 + js - j);
-            }
-            n0 += __shfl(ns, 63);
-            j0 += __shfl(js, 63);
+    if (threadIdx.x < 64) scan(sel.before, a.experts * parts, threadIdx.x);
+    __syncthreads();
+    auto end_of = [&](uint32_t e) { return e + 1 < a.experts ? (uint32_t)sel.before[(e + 1) * parts] : pairs; };
+    for (uint32_t x = threadIdx.x; x < a.experts * parts; x += blockDim.x) {
+        const uint32_t e = x / parts, part = x % parts;
+        if (part == 0) sel.jobs_before[e] = (uint16_t)((end_of(e) - sel.before[x] + a.columns - 1) / a.columns);
+        uint32_t at = sel.before[x];
+        if (at == (x + 1 < a.experts * parts ? (uint32_t)sel.before[x + 1] : pairs)) continue;
+        for (uint32_t q = eights * part / parts; q < eights * (part + 1) / parts; ++q) {
+            const u16x8 v = id8[q];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (v[i] == e) sel.pair[at++] = (uint16_t)(q * 8 + i);
         }
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const uint32_t jobs = scan(sel.jobs_before, a.experts, threadIdx.x);
         if (threadIdx.x == 0) {
-            *table.count = j0;
-            table.first[j0] = (uint16_t)pairs;
+            *table.count = jobs;
+            table.first[jobs] = (uint16_t)pairs;
         }
+    }
+    for (uint32_t i = threadIdx.x; i < pairs; i += blockDim.x) {
+        const uint32_t p = sel.pair[i];
+        table.pair[i] = (uint16_t)p;
+        table.weight[i] = sel.weight[p];
     }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) {
-        const uint32_t from = before[e], to = e + 1 < a.experts ? before[e + 1] : pairs;
-        if (from == to) continue;
-        uint32_t at = from, job = jobs_before[e];
+        const uint32_t from = sel.before[e * parts], to = end_of(e);
+        uint32_t job = sel.jobs_before[e];
         for (uint32_t n = from; n < to; n += a.columns, ++job) {
             table.expert[job] = (uint16_t)e;
             table.first[job] = (uint16_t)n;
         }
-        for (uint32_t p = 0; p < pairs; ++p)
-            if (id[p] == e) {
-                table.pair[at] = (uint16_t)p;
-                table.weight[at++] = weight[p];
-            }
     }
+}
+
+__device__ inline char *table_of_row(const MoeArgs &a, uint32_t row) { return a.table + (uint64_t)row * table_bytes(min(kTokens, a.tokens) * a.top_k, a.most_jobs); }
+
+// A wavefront: the selection of one token.  The work-group of a row that is done last makes the row's table (the counter was cleared by the kernel before).
+constexpr uint32_t kSelectTokens = 4;           // of a work-group
+__global__ void __launch_bounds__(kSelectTokens * 64) moe_select_kernel(const MoeArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ bool last;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.y;
+    const uint32_t token0 = row * kTokens, tokens = min(kTokens, a.tokens - token0), pairs = tokens * a.top_k, most_pairs = min(kTokens, a.tokens) * a.top_k;
+    const uint32_t t = blockIdx.x * kSelectTokens + wave;
+    if (t < tokens) {
+        uint32_t expert;
+        float weight;
+        select_token(a, token0 + t, lane, expert, weight);
+        if (lane < a.top_k) {
+            const uint64_t p = (uint64_t)(token0 + t) * a.top_k + lane;
+            // (through to where every XCD sees them)
+            __hip_atomic_store(a.chosen + p, expert, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(a.chosen_weights + p, weight, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (a.ids) a.ids[p] = (int)expert;
+            if (a.weights) a.weights[p] = weight;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const uint32_t groups = (tokens + kSelectTokens - 1) / kSelectTokens;
+    if (threadIdx.x == 0) last = blockIdx.x < groups && __hip_atomic_fetch_add(a.selected + row, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == groups;
+    __syncthreads();
+    if (!last) return;
+    const Selection sel = selection_at(lds, most_pairs, a.experts);
+    for (uint32_t p = threadIdx.x; p < pairs; p += blockDim.x) {
+        sel.id[p] = (uint16_t)__hip_atomic_load(a.chosen + (uint64_t)token0 * a.top_k + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sel.weight[p] = __hip_atomic_load(a.chosen_weights + (uint64_t)token0 * a.top_k + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    make_table(a, pairs, sel, table_at(table_of_row(a, row), most_pairs, a.most_jobs));
 }
 
 // A row's table, in LDS.
 __device__ inline Table stage_table(const MoeArgs &a, uint32_t row, char *lds)
 {
     const uint32_t most_pairs = min(kTokens, a.tokens) * a.top_k, bytes = table_bytes(most_pairs, a.most_jobs);
-    const char *const from = a.table + (uint64_t)row * bytes;
+    const char *const from = table_of_row(a, row);
     for (uint32_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<u32x4 *>(lds + i) = *reinterpret_cast<const u32x4 *>(from + i);
     __syncthreads();
     return table_at(lds, most_pairs, a.most_jobs);
@@ -294,7 +399,35 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t tiles = (a.inner + 15) / 16, token0 = blockIdx.y * kTokens;
     float *const sums = reinterpret_cast<float *>(lds + waves * S::LDS_BYTES);           // [set][wavefront][tile][..]
-    const Table table = stage_table(a, blockIdx.y, reinterpret_cast<char *>(sums + 2 * waves * SET));
+    char *const table_lds = reinterpret_cast<char *>(sums + 2 * waves * SET);
+    Table table;
+    if constexpr (N2 < 16) {
+        // A few tokens are selected by every work-group for itself, in less than another launch takes; one of them leaves the table to the next kernel.
+        const uint32_t most_pairs = a.tokens * a.top_k;
+        table = table_at(table_lds, most_pairs, a.most_jobs);
+        const Selection sel = selection_at(lds, most_pairs, a.experts);                 // (where the rings will be)
+        for (uint32_t t = wave; t < a.tokens; t += waves) {
+            uint32_t expert;
+            float weight;
+            select_token(a, t, lane, expert, weight);
+            if ((uint32_t)lane < a.top_k) {
+                const uint32_t p = t * a.top_k + lane;
+                sel.id[p] = (uint16_t)expert;
+                sel.weight[p] = weight;
+                if (blockIdx.x == 0 && a.ids) a.ids[p] = (int)expert;
+                if (blockIdx.x == 0 && a.weights) a.weights[p] = weight;
+            }
+        }
+        make_table(a, most_pairs, sel, table);
+        __syncthreads();
+        if (blockIdx.x == 0) {
+            const uint32_t bytes = table_bytes(most_pairs, a.most_jobs);
+            for (uint32_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<u32x4 *>(a.table + i) = *reinterpret_cast<const u32x4 *>(table_lds + i);
+        }
+    } else {
+        table = stage_table(a, blockIdx.y, table_lds);
+    }
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < a.down_tiles; i += gridDim.x * blockDim.x) a.arrived[blockIdx.y * a.down_tiles + i] = 0;
     const uint32_t units = *table.count * tiles;
     const uint32_t unit0 = (uint32_t)((uint64_t)units * blockIdx.x / gridDim.x), unit1 = (uint32_t)((uint64_t)units * (blockIdx.x + 1) / gridDim.x);
     auto enter = [&](uint32_t u, typename S::Job &j) {
@@ -353,6 +486,8 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
 
 // A work-group: 16 * FT elements of y of its tokens: the same rows of down of every expert that was selected, the jobs' blocks one behind the other and shared
 // by the wavefronts.  What a wavefront has of a job goes to its own sums of all tokens; those are added in the order of the wavefronts.
+// Where that is too few work-groups for the chip, several (the grid's z) share the blocks: each leaves its sums in memory, and the one that is done last adds
+// them up, in the order of their numbers.  The counters that tell it were cleared by the kernel before.
 template <typename T, bool W4, int N2, int FT, int FOLDS, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs a)
 {
@@ -398,14 +533,33 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs 
     };
     const uint32_t per_job = S::blocks_of(a.inner);
     S s(a.inner, a.group / kW4Group, 0, per_job, lds + wave * S::LDS_BYTES, lane);
-    const uint32_t blocks = per_job * *table.count, each = blocks / waves, more = blocks % waves;
-    s.run(wave * each + min(wave, more), each + (wave < more), enter, flush);
+    const uint32_t blocks = per_job * *table.count, sharers = waves * gridDim.z, sharer = blockIdx.z * waves + wave, each = blocks / sharers, more = blocks % sharers;
+    s.run(sharer * each + min(sharer, more), each + (sharer < more), enter, flush);
     __syncthreads();
-    for (uint32_t at = threadIdx.x; at < tokens * ROWS; at += blockDim.x) {
+    const uint32_t sums = tokens * ROWS, tile = blockIdx.y * gridDim.x + blockIdx.x;
+    float *const parts = a.parts + (uint64_t)tile * gridDim.z * most_tokens * ROWS;
+    if (gridDim.z > 1) {
+        for (uint32_t at = threadIdx.x; at < sums; at += blockDim.x) {
+            float v = 0.0f;
+            for (uint32_t w = 0; w < waves; ++w) v += all[w * most_tokens * ROWS + at];
+            // (through to where every XCD sees them)
+            __hip_atomic_store(parts + blockIdx.z * most_tokens * ROWS + at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t *const last = reinterpret_cast<uint32_t *>(lds);
+        if (threadIdx.x == 0) *last = __hip_atomic_fetch_add(a.arrived + tile, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.z;
+        __syncthreads();
+        if (!*last) return;
+    }
+    for (uint32_t at = threadIdx.x; at < sums; at += blockDim.x) {
         const uint32_t i = row0 + at % ROWS, t = at / ROWS;
         if (i >= a.hidden) continue;
         float v = 0.0f;
-        for (uint32_t w = 0; w < waves; ++w) v += all[w * most_tokens * ROWS + at];
+        if (gridDim.z > 1)
+            for (uint32_t z = 0; z < gridDim.z; ++z) v += __hip_atomic_load(parts + z * most_tokens * ROWS + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else
+            for (uint32_t w = 0; w < waves; ++w) v += all[w * most_tokens * ROWS + at];
         v *= a.alpha;
         T *y = static_cast<T *>(a.y) + (token0 + t) * a.ldy + i;
         if (a.beta != 0.0f) v = __builtin_fmaf(a.beta, (float)*y, v);
@@ -439,7 +593,8 @@ int check_layer(const mmbo_moe_layer *l)
     return check_matrix(l->down, l->inner, l->group);
 }
 
-size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+// (whole memory lines: rows of h that share lines with others cost the last product 74 us instead of 60, 64 tokens of 16 x 4096 x 2048)
+size_t lines(size_t n) { return (n + 127) / 128 * 128; }
 
 // Columns side by side in a stream for so many tokens, and the most jobs that a row of them can make: every job but an expert's last is full.
 uint32_t columns_of(uint32_t tokens) { return tokens == 1 ? 1 : tokens <= 4 ? 4 : 16; }
@@ -449,18 +604,33 @@ uint32_t most_jobs_of(const mmbo_moe_layer &l, size_t tokens)
     return std::min<uint32_t>(pairs, (uint32_t)l.experts + pairs / columns_of((uint32_t)tokens));
 }
 
+// Work-groups that share a tile of y: as many as make one for each of 256 CUs, up to eight.
+constexpr size_t kDownRows = 16;
+uint32_t sharers_of(const mmbo_moe_layer &l, size_t tokens)
+{
+    const size_t tiles = ceil_div(l.hidden, kDownRows) * ceil_div(tokens, kTokens);
+    return (uint32_t)std::min<size_t>(std::max<size_t>(256 / tiles, 1), 8);
+}
+
 // Places of the workspace's parts, in bytes.
 struct Parts {
-    size_t logits, table, h, all, ld_h;
+    size_t logits, table, chosen, chosen_weights, selected, arrived, parts, h, all, ld_h;
 };
 Parts parts_of(const mmbo_moe_layer &l, size_t tokens)
 {
     Parts p;
-    p.ld_h = (l.inner + 7) / 8 * 8;
+    p.ld_h = (l.inner + 63) / 64 * 64;
     p.logits = 0;
-    p.table = p.logits + round16(tokens * l.experts * sizeof(double));
-    p.h = p.table + ceil_div(tokens, kTokens) * table_bytes((uint32_t)(std::min<size_t>(tokens, kTokens) * l.top_k), most_jobs_of(l, tokens));
-    p.all = p.h + round16(2 * tokens * l.top_k * p.ld_h * sizeof(half_t));
+    p.table = p.logits + lines(tokens * l.experts * sizeof(double));
+    p.chosen = p.table + lines(ceil_div(tokens, kTokens) * table_bytes((uint32_t)(std::min<size_t>(tokens, kTokens) * l.top_k), most_jobs_of(l, tokens)));
+    const size_t tiles = ceil_div(l.hidden, kDownRows) * ceil_div(tokens, kTokens);
+    p.chosen_weights = p.chosen + lines(tokens * l.top_k * sizeof(uint32_t));
+    p.selected = p.chosen_weights + lines(tokens * l.top_k * sizeof(float));
+    p.arrived = p.selected + lines(ceil_div(tokens, kTokens) * sizeof(uint32_t));
+    p.parts = p.arrived + lines(tiles * sizeof(uint32_t));
+    const uint32_t sharers = sharers_of(l, std::max<size_t>(tokens, 1));
+    p.h = p.parts + lines(sharers > 1 ? tiles * sharers * std::min<size_t>(tokens, kTokens) * kDownRows * sizeof(float) : 0);
+    p.all = p.h + lines(2 * tokens * l.top_k * p.ld_h * sizeof(half_t));
     return p;
 }
 
@@ -491,7 +661,7 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
 template <typename T, bool W4, int N2, int FOLDS, bool ZEROS>
 hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
 {
-    constexpr int UP_DEPTH = N2 < 16 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = 1;
+    constexpr int UP_DEPTH = N2 < 16 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
     typedef stream::Stream<T, W4, N2, 2, 1, FOLDS, ZEROS, UP_DEPTH> Up;
     typedef stream::Stream<T, W4, N2, FT, 2, FOLDS, ZEROS, DEPTH> Down;
     const uint32_t rows = (uint32_t)ceil_div(a.tokens, kTokens), most_tokens = std::min(a.tokens, kTokens);
@@ -506,7 +676,7 @@ hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
     const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), 256);
     hipError_t e = launch_args(up, dim3(groups, rows), dim3(up_waves * 64), up_waves * up_wave + table, s, a);
     if (e != hipSuccess) return e;
-    return launch_args(down, dim3((unsigned)ceil_div(a.hidden, 16 * FT), rows), dim3(down_waves * 64), down_waves * down_wave + table, s, a);
+    return launch_args(down, dim3(a.down_tiles, rows, a.sharers), dim3(down_waves * 64), down_waves * down_wave + table, s, a);
 }
 
 template <typename T, int N2>
@@ -521,16 +691,6 @@ hipError_t launch_columns(const MoeArgs &a, hipStream_t s)
     return folds(std::integral_constant<int, 4>());
 }
 
-hipError_t launch_select(const MoeArgs &a, hipStream_t s)
-{
-    const uint32_t most_tokens = std::min(a.tokens, kTokens), rows = (uint32_t)ceil_div(a.tokens, kTokens);
-    const unsigned waves = std::min(most_tokens, 16u), lds = most_tokens * a.top_k * 6 + a.experts * 4;
-    const dim3 block(waves * 64);
-    if (a.experts <= 64) return launch_args(moe_select_kernel<1>, dim3(rows), block, lds, s, a);
-    if (a.experts <= 128) return launch_args(moe_select_kernel<2>, dim3(rows), block, lds, s, a);
-    return launch_args(moe_select_kernel<8>, dim3(rows), block, lds, s, a);
-}
-
 template <typename T>
 hipError_t run(const MoeArgs &a, bool router32, hipStream_t s)
 {
@@ -538,8 +698,12 @@ hipError_t run(const MoeArgs &a, bool router32, hipStream_t s)
     hipError_t e = router32 ? launch_args(moe_logits_kernel<T, float>, logits, dim3(256), 0, s, a)
                             : launch_args(moe_logits_kernel<T, T>, logits, dim3(256), 0, s, a);
     if (e != hipSuccess) return e;
-    e = launch_select(a, s);
-    if (e != hipSuccess) return e;
+    if (a.columns >= 16) {
+        const uint32_t most_tokens = std::min(a.tokens, kTokens);
+        e = launch_args(moe_select_kernel, dim3((unsigned)ceil_div(most_tokens, kSelectTokens), (unsigned)ceil_div(a.tokens, kTokens)), dim3(kSelectTokens * 64),
+                        select_bytes(most_tokens * a.top_k, a.experts), s, a);
+        if (e != hipSuccess) return e;
+    }
     return a.columns == 1 ? launch_columns<T, 1>(a, s) : a.columns == 4 ? launch_columns<T, 4>(a, s) : launch_columns<T, 16>(a, s);
 }
 
@@ -553,7 +717,9 @@ extern "C" {
 size_t mmbo_moe_workspace_bytes(const mmbo_moe_layer *layer, size_t tokens)
 {
     if (check_layer(layer) != MMBO_OK || tokens > MMBO_MOE_MAX_TOKENS) return 0;
-    return std::max<size_t>(parts_of(*layer, tokens).all, 16);
+    size_t most = 16;                           // (fewer tokens may need more: they are laid out in other tiles and jobs)
+    for (size_t t = 1; t <= tokens; ++t) most = std::max(most, parts_of(*layer, t).all);
+    return most;
 }
 
 int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, const void *x, size_t ldx, const void *beta, void *y,
@@ -579,6 +745,13 @@ int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, cons
     a.h = ws + p.h;
     a.ld_h = (uint32_t)p.ld_h;
     a.table = ws + p.table;
+    a.chosen = reinterpret_cast<uint32_t *>(ws + p.chosen);
+    a.chosen_weights = reinterpret_cast<float *>(ws + p.chosen_weights);
+    a.selected = reinterpret_cast<uint32_t *>(ws + p.selected);
+    a.arrived = reinterpret_cast<uint32_t *>(ws + p.arrived);
+    a.parts = reinterpret_cast<float *>(ws + p.parts);
+    a.down_tiles = (uint32_t)ceil_div(l.hidden, kDownRows);
+    a.sharers = sharers_of(l, tokens);
     a.ids = ids;
     a.weights = weights;
     a.columns = columns_of((uint32_t)tokens);

@@ -23,64 +23,127 @@ template <typename TW>
 __device__ inline float finite(float w)
 {
     const float most = Limits<TW>::largest;
-    return w != w ? 0.0f : fminf(fmaxf(w, -most), most);
+    return w != w ? 0.0f : __builtin_amdgcn_fmed3f(w, -most, most);
 }
 
-// The whole number nearest to w / s, halves to even, for numbers within 16 or clamped there: the quotient's rounding may pick the wrong one next to
-// a border, and the remainder w - n * s, which is exact in fp32, says so.
-__device__ inline float nearest(float w, float s)
+// The whole number nearest to w / s, halves to even, for numbers within 16 or clamped there; by = 1 / s.  The product's rounding may pick the wrong one next to a
+// border; the remainder w - n * s, which is exact in fp32, says so.
+__device__ inline float nearest(float w, float s, float by)
 {
-    float n = rintf(fminf(fmaxf(w / s, -16.0f), 16.0f));
+    float n = rintf(__builtin_amdgcn_fmed3f(w * by, -16.0f, 16.0f));
     const float r = __builtin_fmaf(-n, s, w), half = 0.5f * s;
-    const bool odd = ((int)n & 1) != 0;
-    if (r > half || (r == half && odd)) n += 1.0f;
-    else if (r < -half || (r == -half && odd)) n -= 1.0f;
+    if (__builtin_fabsf(r) >= half) {                               // (rare)
+        const bool odd = ((int)n & 1) != 0;
+        if (r > half || (r == half && odd)) n += 1.0f;
+        else if (r < -half || (r == -half && odd)) n -= 1.0f;
+    }
     return n;
 }
 
-// One thread: one group of one row.
-template <typename TW, typename T>
+// Sixteen bytes or the elements of them that exist (here >= 1), as floats in the format's sense; the others are 0.
+template <typename TW> constexpr int kPer16 = 16 / (int)sizeof(TW);
+template <typename TW>
+__device__ inline void load_weights(float (&v)[kPer16<TW>], const TW *p, int64_t here)
+{
+    typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+    union { u32x4 q; TW e[kPer16<TW>]; } u;
+    if (here >= kPer16<TW>) {
+        u.q = *reinterpret_cast<const u32x4_any *>(p);
+    } else {
+        u.q = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kPer16<TW> - 1; ++i)
+            if (i < here) u.e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kPer16<TW>; ++i) v[i] = finite<TW>((float)u.e[i]);
+}
+
+// LANES lanes, neighbours, have a group of a row: each 16 bytes of it a step.  Groups of up to 64 * 16 bytes go by in one step and are read once; longer ones are
+// read twice, the second time from the cache.  Bound by what it reads and writes.
+template <typename TW, typename T, int LANES>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
 {
-    const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (uint64_t)a.m * a.groups) return;
+    constexpr int E = kPer16<TW>;
+    const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES, all = (uint64_t)a.m * a.groups;
+    const uint32_t lane = threadIdx.x % LANES;
+    if (at >= all) return;                                          // (the lanes of a group together)
     const uint64_t i = at / a.groups;
-    const uint32_t g = (uint32_t)(at % a.groups);
+    const uint32_t g = (uint32_t)(at - i * a.groups);
     const uint64_t l0 = (uint64_t)g * a.group, l1 = l0 + a.group < a.k ? l0 + a.group : a.k;
     const TW *w = static_cast<const TW *>(a.W) + i * a.ldw;
-    float low = 0.0f, high = 0.0f;
-    for (uint64_t l = l0; l < l1; ++l) {
-        const float v = finite<TW>((float)w[l]);
-        low = fminf(low, v);
-        high = fmaxf(high, v);
+    float low = 0.0f, high = 0.0f, v[E];
+    for (uint64_t l = l0 + lane * E; l < l1; l += LANES * E) {
+        load_weights<TW>(v, w + l, (int64_t)(l1 - l));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            low = fminf(low, v[e]);
+            high = fmaxf(high, v[e]);
+        }
+    }
+    for (int d = 1; d < LANES; d <<= 1) {
+        low = fminf(low, __shfl_xor(low, d));
+        high = fmaxf(high, __shfl_xor(high, d));
     }
     const bool zeros = a.w.zeros != nullptr;
     // (in 64 bits: high - low may pass the largest float)
     float s = zeros ? (float)(((double)high - (double)low) / 15.0) : fmaxf(high, -low) / 7.0f;
     s = (float)(T)fminf(s, Limits<T>::largest);
     float z = zeros ? 0.0f : kW4Zero;
-    if (zeros && s != 0.0f) z = fminf(fmaxf(nearest(-low, s), 0.0f), 15.0f);
-    static_cast<T *>(const_cast<void *>(a.w.scales))[g + i * a.w.lds] = (T)s;
-    if (zeros) const_cast<uint8_t *>(a.w.zeros)[g + i * a.w.ldz] = (uint8_t)z;
+    // (scales so small that 1 / s is infinite: as everything by 2^64, which changes no quotient)
+    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, by = 1.0f / su;
+    if (zeros && s != 0.0f) z = fminf(fmaxf(nearest(-low * up, su, by), 0.0f), 15.0f);
+    if (lane == 0) {
+        static_cast<T *>(const_cast<void *>(a.w.scales))[g + i * a.w.lds] = (T)s;
+        if (zeros) const_cast<uint8_t *>(a.w.zeros)[g + i * a.w.ldz] = (uint8_t)z;
+    }
     uint8_t *q = const_cast<uint8_t *>(a.w.q) + i * a.w.ldq;
-    for (uint64_t l = l0; l < l1; l += 2) {
-        uint32_t code[2] = {0, 0};
-        for (int e = 0; e < 2; ++e)
-            if (l + e < l1) code[e] = (uint32_t)(s == 0.0f ? z : fminf(fmaxf(nearest(finite<TW>((float)w[l + e]), s) + z, 0.0f), 15.0f));
-        q[l / 2] = (uint8_t)(code[0] | code[1] << 4);
+    const bool once = l1 - l0 <= LANES * E;
+    for (uint64_t l = l0 + lane * E; l < l1; l += LANES * E) {
+        if (!once) load_weights<TW>(v, w + l, (int64_t)(l1 - l));
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t code = (uint32_t)(s == 0.0f ? z : __builtin_amdgcn_fmed3f(nearest(v[e] * up, su, by) + z, 0.0f, 15.0f));
+            if (l + e < l1) codes |= code << (4 * e);
+        }
+        const uint32_t bytes = (uint32_t)((l1 - l < E ? l1 - l : E) + 1) / 2;
+        typedef uint32_t __attribute__((aligned(1))) u32_any;
+        typedef uint16_t __attribute__((aligned(1))) u16_any;
+        if (bytes == E / 2) {
+            if constexpr (E == 8) *reinterpret_cast<u32_any *>(q + l / 2) = codes;
+            else *reinterpret_cast<u16_any *>(q + l / 2) = (uint16_t)codes;
+        } else {
+            for (uint32_t b = 0; b < bytes; ++b) q[l / 2 + b] = (uint8_t)(codes >> (8 * b));
+        }
     }
 }
 
+// A thread: 32 places of a row, with one scale.
 template <typename T>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
 {
+    const uint32_t pieces = (a.k + 31) / 32;
     const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (uint64_t)a.m * a.k) return;
-    const uint64_t i = at / a.k, l = at % a.k;
-    const uint32_t g = (uint32_t)(l / a.group);
-    const uint8_t byte = a.w.q[i * a.w.ldq + l / 2];
-    const float z = a.w.zeros ? (float)(a.w.zeros[g + i * a.w.ldz] & kW4ZeroMask) : kW4Zero;
-    static_cast<T *>(a.W)[i * a.ldw + l] = (T)(((float)(l & 1 ? byte >> 4 : byte & 15) - z) * load_scale<T>(a.w.scales, g + i * a.w.lds));
+    if (at >= (uint64_t)a.m * pieces * 4) return;
+    // (four threads to a piece, eight places each: 64 bytes of W leave together)
+    const uint64_t piece = at >> 2, i = piece / pieces;
+    const uint32_t p = (uint32_t)(piece - i * pieces), g = p * 32 / a.group, l = p * 32 + (uint32_t)(at & 3) * 8;
+    if (l >= a.k) return;
+    const float z = a.w.zeros ? (float)(a.w.zeros[g + i * a.w.ldz] & kW4ZeroMask) : kW4Zero, s = load_scale<T>(a.w.scales, g + i * a.w.lds);
+    const uint8_t *q = a.w.q + i * a.w.ldq + l / 2;
+    T *to = static_cast<T *>(a.W) + i * a.ldw + l;
+    union { u32x4 v; T e[8]; } u;
+    typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+    typedef uint32_t __attribute__((aligned(1))) u32_any;
+    if (l + 8 <= a.k) {
+        const uint32_t codes = *reinterpret_cast<const u32_any *>(q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u.e[e] = (T)(((float)(codes >> (4 * e) & 15) - z) * s);
+        *reinterpret_cast<u32x4_any *>(to) = u.v;
+    } else {
+        for (uint32_t e = 0; l + e < a.k; ++e) to[e] = (T)(((float)(e & 1 ? q[e / 2] >> 4 : q[e / 2] & 15) - z) * s);
+    }
 }
 
 constexpr size_t kMaxDim = 0x7FFFFFFFull;
@@ -102,6 +165,16 @@ W4Matrix matrix_of(const void *Q, size_t ldq, const void *scales, size_t lds, co
 }
 
 int status_of(hipError_t e) { return e == hipSuccess ? MMBO_OK : report_hip_error(e); }
+
+// launch(first row, rows) over all rows, so many at a time that their threads, `threads` a row, are fewer than the 2^32 of a grid.
+template <typename Launch>
+int by_rows(size_t m, size_t threads, const Launch &launch)
+{
+    const size_t most = std::max<size_t>((1ull << 31) / threads, 1);
+    for (size_t i = 0; i < m; i += most)
+        if (hipError_t e = launch(i, std::min(m - i, most))) return report_hip_error(e);
+    return MMBO_OK;
+}
 
 template <typename Kernel>
 hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
@@ -207,19 +280,33 @@ int mmbo_w4_quantize(int w_dtype, int dtype, size_t m, size_t k, size_t group, c
     if (ldw > kMaxDim || ldw < k) return MMBO_ERR_INVALID_SIZE;
     if (m == 0 || k == 0) return MMBO_OK;
     if (!W || !Q || !scales) return MMBO_ERR_NULL_POINTER;
-    const size_t groups = (k + group - 1) / group, blocks = (m * groups + 255) / 256;
-    if (blocks > kMaxDim) return MMBO_ERR_INVALID_SIZE;
-    const QuantArgs a{matrix_of(Q, ldq, scales, lds, zeros, ldz), const_cast<void *>(W), ldw, (uint32_t)m, (uint32_t)k, (uint32_t)group, (uint32_t)groups};
+    const size_t groups = ceil_div(k, group);
+    QuantArgs a{matrix_of(Q, ldq, scales, lds, zeros, ldz), const_cast<void *>(W), ldw, 0, (uint32_t)k, (uint32_t)group, (uint32_t)groups};
     hipStream_t s = static_cast<hipStream_t>(stream);
+    // lanes for a group of any size, as many as its 16 bytes: a power of two
+    const size_t wsize = w_dtype == MMBO_F32 ? 4 : 2, pieces = ceil_div(std::min(group, k) * wsize, 16);
+    int lanes = 4;
+    while (lanes < 64 && (size_t)lanes < pieces) lanes *= 2;
     auto launch = [&](auto *w, auto *t) {
         using TW = std::remove_pointer_t<decltype(w)>;
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_args(w4_quantize_kernel<TW, T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)ceil_div(a.m * groups * lanes, 256)), block(256);
+        return lanes == 4    ? launch_args(w4_quantize_kernel<TW, T, 4>, grid, block, 0, s, a)
+               : lanes == 8  ? launch_args(w4_quantize_kernel<TW, T, 8>, grid, block, 0, s, a)
+               : lanes == 16 ? launch_args(w4_quantize_kernel<TW, T, 16>, grid, block, 0, s, a)
+               : lanes == 32 ? launch_args(w4_quantize_kernel<TW, T, 32>, grid, block, 0, s, a)
+                             : launch_args(w4_quantize_kernel<TW, T, 64>, grid, block, 0, s, a);
     };
     auto by_weight = [&](auto *t) {
         return w_dtype == MMBO_F32 ? launch((float *)nullptr, t) : w_dtype == MMBO_F16 ? launch((half_t *)nullptr, t) : launch((bf16_t *)nullptr, t);
     };
-    return status_of(dtype == MMBO_F16 ? by_weight((half_t *)nullptr) : by_weight((bf16_t *)nullptr));
+    const size_t esz = 2;
+    return by_rows(m, groups * lanes, [&](size_t i, size_t rows) {
+        a.m = (uint32_t)rows;
+        a.W = const_cast<char *>(static_cast<const char *>(W)) + i * ldw * wsize;
+        a.w = matrix_of(static_cast<const char *>(Q) + i * (ldq / 2), ldq, static_cast<const char *>(scales) + i * lds * esz, lds, zeros ? zeros + i * ldz : nullptr, ldz);
+        return dtype == MMBO_F16 ? by_weight((half_t *)nullptr) : by_weight((bf16_t *)nullptr);
+    });
 }
 
 int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *Q, size_t ldq, const void *scales, size_t lds,
@@ -230,12 +317,17 @@ int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *
     if (ldw > kMaxDim || ldw < k) return MMBO_ERR_INVALID_SIZE;
     if (m == 0 || k == 0) return MMBO_OK;
     if (!W || !Q || !scales) return MMBO_ERR_NULL_POINTER;
-    const size_t blocks = (m * k + 255) / 256;
-    if (blocks > kMaxDim) return MMBO_ERR_INVALID_SIZE;
-    const QuantArgs a{matrix_of(Q, ldq, scales, lds, zeros, ldz), W, ldw, (uint32_t)m, (uint32_t)k, (uint32_t)group, (uint32_t)((k + group - 1) / group)};
+    QuantArgs a{matrix_of(Q, ldq, scales, lds, zeros, ldz), W, ldw, 0, (uint32_t)k, (uint32_t)group, (uint32_t)ceil_div(k, group)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return status_of(dtype == MMBO_F16 ? launch_args(w4_dequantize_kernel<half_t>, dim3((unsigned)blocks), dim3(256), 0, s, a)
-                                       : launch_args(w4_dequantize_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, s, a));
+    const size_t threads = ceil_div(k, 32) * 4, esz = 2;
+    return by_rows(m, threads, [&](size_t i, size_t rows) {
+        a.m = (uint32_t)rows;
+        a.W = static_cast<char *>(W) + i * ldw * esz;
+        a.w = matrix_of(static_cast<const char *>(Q) + i * (ldq / 2), ldq, static_cast<const char *>(scales) + i * lds * esz, lds, zeros ? zeros + i * ldz : nullptr, ldz);
+        const dim3 grid((unsigned)ceil_div(rows * threads, 256));
+        return dtype == MMBO_F16 ? launch_args(w4_dequantize_kernel<half_t>, grid, dim3(256), 0, s, a)
+                                 : launch_args(w4_dequantize_kernel<bf16_t>, grid, dim3(256), 0, s, a);
+    });
 }
 
 }  // extern "C"

@@ -61,6 +61,14 @@ def test_calls_that_are_refused():
     assert _status(layer, tokens=0, x=None, y=None, workspace=None) == 0
 
 
+@pytest.mark.parametrize("change", [dict(hidden=2048, ld_router=2048), dict(experts=32, top_k=32), dict(hidden=16, ld_router=64, experts=512, top_k=32)])
+def test_a_workspace_serves_fewer_tokens_too(change):
+    h = change.get("hidden", 64)
+    layer = _layer(gate_up=G.moe_matrix(16, h, 64 * h), down=G.moe_matrix(16, 32, 32 * h), **change)
+    sizes = [G.moe_workspace_bytes(layer, t) for t in range(G.MOE_MAX_TOKENS + 1)]
+    assert sizes == sorted(sizes) and all(n % 16 == 0 for n in sizes)
+
+
 # ---- on the GPU
 
 class Problem:
