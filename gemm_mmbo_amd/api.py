@@ -60,7 +60,9 @@ class MoeLayer(ctypes.Structure):
 
 _lib = None
 try:
-    from . import _frontend             # the GEMM front-ends without ctypes (csrc/frontend.cc); without it they are the functions below
+    from . import _frontend             # the front-ends without ctypes (csrc/frontend.cc); without it they are the functions below
+    if not hasattr(_frontend, "moe"):   # (built from older sources: the next build replaces it)
+        _frontend = None
 except ImportError:
     _frontend = None
 
@@ -130,7 +132,7 @@ def lib():
         L.mmbo_version.restype = ctypes.c_char_p
         if _frontend is not None:
             _frontend.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in
-                             (L.mmbo_gemm, L.mmbo_gemm_strided_batched, L.mmbo_gemm_strided_batched_static_workspace)))
+                             (L.mmbo_gemm, L.mmbo_gemm_strided_batched, L.mmbo_gemm_strided_batched_static_workspace, L.mmbo_gemm_w4, L.mmbo_moe)))
         _lib = L
     return _lib
 
@@ -192,14 +194,6 @@ def gemm_strided_batched_static_workspace(dtype, transA, transB, m, n, k, alpha,
                                                             _stream_handle(stream)))
 
 
-_PYTHON_FRONT_ENDS = (gemm, gemm_strided_batched, gemm_strided_batched_static_workspace)
-if _frontend is not None:
-    # plain calls go straight to the C ABI, all others to the functions above
-    _frontend.setup(*_PYTHON_FRONT_ENDS, _check)
-    gemm, gemm_strided_batched = _frontend.gemm, _frontend.gemm_strided_batched
-    gemm_strided_batched_static_workspace = _frontend.gemm_strided_batched_static_workspace
-
-
 def gemm_w4(dtype, m, n, k, group, alpha, Q, ldq, scales, lds, zeros, ldz, B, ldb, beta, C, ldc, stream=None):
     """C = alpha*W*B + beta*C with W of m rows and k columns in 4 bits (the format: include/mmbo_gemm.h): codes Q, ldq codes from row to row, a
     scale and a zero point (zeros None: 8) for every `group` codes of a row.  dtype F16 or BF16: scales, B, C."""
@@ -251,6 +245,15 @@ def moe(layer, tokens, alpha, x, ldx, beta, y, ldy, workspace, workspace_bytes, 
     al, be = _scalars(F32, alpha, beta)
     _check(lib().mmbo_moe(ctypes.byref(layer), tokens, ctypes.byref(al), _devptr(x), ldx, ctypes.byref(be), _devptr(y), ldy, _devptr(ids),
                           _devptr(weights), _devptr(workspace), workspace_bytes, _stream_handle(stream)))
+
+
+_PYTHON_FRONT_ENDS = (gemm, gemm_strided_batched, gemm_strided_batched_static_workspace, gemm_w4, moe)
+if _frontend is not None:
+    # plain calls go straight to the C ABI, all others to the functions above
+    _frontend.setup(*_PYTHON_FRONT_ENDS, _check, MoeLayer)
+    gemm, gemm_strided_batched = _frontend.gemm, _frontend.gemm_strided_batched
+    gemm_strided_batched_static_workspace = _frontend.gemm_strided_batched_static_workspace
+    gemm_w4, moe = _frontend.gemm_w4, _frontend.moe
 
 
 def static_workspace_bytes():

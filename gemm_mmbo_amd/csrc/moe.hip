@@ -372,34 +372,29 @@ __device__ inline Table stage_table(const MoeArgs &a, uint32_t row, char *lds)
 constexpr int kMoeWaves = 8;                    // or as many as fit the LDS
 constexpr unsigned kLds = 160 * 1024;
 
-// A row of an expert's weight for the lanes of a job.
+// The scales of an expert's row for the lanes of a job.
 template <typename T, bool W4, bool ZEROS, typename Job>
-__device__ inline void weight_row(Job &j, int f, const MoeMatrix &m, uint32_t expert, uint64_t load_row, uint64_t row)
+__device__ inline void scale_row(Job &j, int f, const MoeMatrix &m, uint32_t expert, uint64_t row)
 {
-    j.w[f] = m.w4.q + (int64_t)expert * m.stride + load_row * m.w4.ldq;
     if constexpr (W4) {
         j.scales[f] = static_cast<const T *>(m.w4.scales) + (int64_t)expert * m.stride_scales + row * m.w4.lds;
         if constexpr (ZEROS) j.zeros[f] = m.w4.zeros + (int64_t)expert * m.stride_zeros + row * m.w4.ldz;
     }
 }
 
-// Of a unit's 16 x 16 sums the columns that N2 leaves: floats of a tile, and where lane l's four lie.
-template <int N2> constexpr int kTileFloats = N2 < 16 ? 16 * N2 : 256;
-
 // A unit of work: h of one job, 16 of its elements: 16 rows of gate and the same of up, `hidden` shared by the wavefronts.  A work-group takes a run of units, one
 // behind the other without a pause in its loads: the wavefronts meet once a unit, over two sets of sums in turn.
-template <typename T, bool W4, int N2, int FOLDS, bool ZEROS, int DEPTH>
+template <typename T, bool W4, int N2, int FOLD, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeArgs a)
 {
     using namespace stream;
-    typedef Stream<T, W4, N2, 2, 1, FOLDS, ZEROS, DEPTH> S;
-    constexpr int NT = S::NT, TILE = kTileFloats<N2>, SET = NT * 2 * TILE;
+    typedef Stream<T, W4, N2, 2, 1, FOLD, ZEROS, DEPTH> S;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t tiles = (a.inner + 15) / 16, token0 = blockIdx.y * kTokens;
     float *const sums = reinterpret_cast<float *>(lds + waves * S::LDS_BYTES);           // [set][wavefront][tile][..]
-    char *const table_lds = reinterpret_cast<char *>(sums + 2 * waves * SET);
+    char *const table_lds = reinterpret_cast<char *>(sums + 2 * waves * S::SET_FLOATS);
     Table table;
     if constexpr (N2 < 16) {
         // A few tokens are selected by every work-group for itself, in less than another launch takes; one of them leaves the table to the next kernel.
@@ -433,39 +428,30 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
     auto enter = [&](uint32_t u, typename S::Job &j) {
         const uint32_t job = (unit0 + u) / tiles, row0 = (unit0 + u) % tiles * 16;
         const uint32_t expert = table.expert[job], first = table.first[job], columns = table.first[job + 1] - first;
-        const uint32_t load_row = min(row0 + (lane >> 2), a.inner - 1), row = min(row0 + (lane & 15), a.inner - 1);
-        weight_row<T, W4, ZEROS>(j, 0, a.gate_up, expert, load_row, row);
-        weight_row<T, W4, ZEROS>(j, 1, a.gate_up, expert, (uint64_t)a.inner + load_row, (uint64_t)a.inner + row);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            const uint32_t col = (uint32_t)(lane >> 2) % N2 % 16 + c * 16;
-            j.x_here[c] = col < columns;
-            j.x[0][c] = static_cast<const T *>(a.x) + (token0 + table.pair[first + min(col, columns - 1)] / a.top_k) * a.ldx;
+        for (int f = 0; f < 2; ++f) {            // gate, up
+            const uint64_t part = (uint64_t)f * a.inner;
+#pragma unroll
+            for (int q = 0; q < S::WP; ++q)
+                j.w[f][q] = a.gate_up.w4.q + (int64_t)expert * a.gate_up.stride + (part + min(row0 + S::load_row(lane, q), a.inner - 1)) * a.gate_up.w4.ldq;
+            scale_row<T, W4, ZEROS>(j, f, a.gate_up, expert, part + min(row0 + (lane & 15), a.inner - 1));
+        }
+#pragma unroll
+        for (int q = 0; q < S::XP; ++q) {
+            const uint32_t col = S::load_column(lane, q);
+            j.x_here[q] = col < columns;
+            j.x[0][q] = static_cast<const T *>(a.x) + (token0 + table.pair[first + min(col, columns - 1)] / a.top_k) * a.ldx;
         }
     };
     auto flush = [&](uint32_t u, const typename S::Sums &acc) {
-        float *const set = sums + (u & 1) * waves * SET;
-        if (N2 >= 16 || lane < 16) {
-#pragma unroll
-            for (int t = 0; t < NT * 2; ++t) {
-                const f32x4 v = acc[t / 2][t % 2];
-                float *const to = set + wave * SET + t * TILE;
-                if constexpr (N2 == 1) to[lane] = v[0];
-                else *reinterpret_cast<f32x4 *>(to + lane * 4) = v;
-            }
-        }
-        // (not __syncthreads(): what is under way for the next unit stays so)
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        float *const set = sums + (u & 1) * waves * S::SET_FLOATS;
+        S::put(set + wave * S::SET_FLOATS, acc, lane);
+        S::meet();
         const uint32_t job = (unit0 + u) / tiles, row0 = (unit0 + u) % tiles * 16, first = table.first[job], columns = table.first[job + 1] - first;
         for (uint32_t at = threadIdx.x; at < N2 * 16; at += blockDim.x) {
             const uint32_t i = row0 + (at & 15), col = at >> 4;
             if (i >= a.inner || col >= columns) continue;
-            const uint32_t place = N2 == 1 ? at & 15 : (col >> 4) * 2 * TILE + ((col >> 2 & 3) * 16 + (at & 15)) * 4 + (col & 3);
-            float g = 0.0f, up = 0.0f;
-            for (uint32_t w = 0; w < waves; ++w) {
-                g += set[w * SET + place];
-                up += set[w * SET + TILE + place];
-            }
+            const float g = S::total(set, 0, at & 15, col, waves), up = S::total(set, 1, at & 15, col, waves);
             const float h = g / (1.0f + expf(-g)) * up;
             T *const to = static_cast<T *>(a.h) + ((uint64_t)token0 * a.top_k + table.pair[first + col]) * a.ld_h + i;
             const T high = (T)h;
@@ -488,11 +474,11 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
 // by the wavefronts.  What a wavefront has of a job goes to its own sums of all tokens; those are added in the order of the wavefronts.
 // Where that is too few work-groups for the chip, several (the grid's z) share the blocks: each leaves its sums in memory, and the one that is done last adds
 // them up, in the order of their numbers.  The counters that tell it were cleared by the kernel before.
-template <typename T, bool W4, int N2, int FT, int FOLDS, bool ZEROS, int DEPTH>
+template <typename T, bool W4, int N2, int FT, int FOLD, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs a)
 {
     using namespace stream;
-    typedef Stream<T, W4, N2, FT, 2, FOLDS, ZEROS, DEPTH> S;
+    typedef Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> S;
     constexpr int NT = S::NT, ROWS = 16 * FT;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63;
@@ -505,15 +491,19 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs 
     auto enter = [&](uint32_t job, typename S::Job &j) {
         const uint32_t expert = table.expert[job], first = table.first[job], columns = table.first[job + 1] - first;
 #pragma unroll
-        for (int f = 0; f < FT; ++f)
-            weight_row<T, W4, ZEROS>(j, f, a.down, expert, min(row0 + f * 16 + (lane >> 2), a.hidden - 1), min(row0 + f * 16 + (lane & 15), a.hidden - 1));
+        for (int f = 0; f < FT; ++f) {
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            const uint32_t col = (uint32_t)(lane >> 2) % N2 % 16 + c * 16;
-            j.x_here[c] = col < columns;
+            for (int q = 0; q < S::WP; ++q)
+                j.w[f][q] = a.down.w4.q + (int64_t)expert * a.down.stride + (uint64_t)min(row0 + f * 16 + S::load_row(lane, q), a.hidden - 1) * a.down.w4.ldq;
+            scale_row<T, W4, ZEROS>(j, f, a.down, expert, min(row0 + f * 16 + (lane & 15), a.hidden - 1));
+        }
+#pragma unroll
+        for (int q = 0; q < S::XP; ++q) {
+            const uint32_t col = S::load_column(lane, q);
+            j.x_here[q] = col < columns;
             const T *h = static_cast<const T *>(a.h) + ((uint64_t)token0 * a.top_k + table.pair[first + min(col, columns - 1)]) * a.ld_h;
-            j.x[0][c] = h;
-            j.x[1][c] = h + (uint64_t)a.tokens * a.top_k * a.ld_h;
+            j.x[0][q] = h;
+            j.x[1][q] = h + (uint64_t)a.tokens * a.top_k * a.ld_h;
         }
     };
     auto flush = [&](uint32_t job, const typename S::Sums &acc) {
@@ -658,20 +648,20 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
     return e;
 }
 
-template <typename T, bool W4, int N2, int FOLDS, bool ZEROS>
+template <typename T, bool W4, int N2, int FOLD, bool ZEROS>
 hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
 {
     constexpr int UP_DEPTH = N2 < 16 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
-    typedef stream::Stream<T, W4, N2, 2, 1, FOLDS, ZEROS, UP_DEPTH> Up;
-    typedef stream::Stream<T, W4, N2, FT, 2, FOLDS, ZEROS, DEPTH> Down;
+    typedef stream::Stream<T, W4, N2, 2, 1, FOLD, ZEROS, UP_DEPTH> Up;
+    typedef stream::Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> Down;
     const uint32_t rows = (uint32_t)ceil_div(a.tokens, kTokens), most_tokens = std::min(a.tokens, kTokens);
     const unsigned table = table_bytes(most_tokens * a.top_k, a.most_jobs);
     static std::atomic<bool> set[2][64];
-    auto up = moe_gate_up_kernel<T, W4, N2, FOLDS, ZEROS, UP_DEPTH>;
-    auto down = moe_down_kernel<T, W4, N2, FT, FOLDS, ZEROS, DEPTH>;
+    auto up = moe_gate_up_kernel<T, W4, N2, FOLD, ZEROS, UP_DEPTH>;
+    auto down = moe_down_kernel<T, W4, N2, FT, FOLD, ZEROS, DEPTH>;
     if (hipError_t e = allow_lds(up, set[0])) return e;
     if (hipError_t e = allow_lds(down, set[1])) return e;
-    const unsigned up_wave = Up::LDS_BYTES + 2 * Up::NT * 2 * kTileFloats<N2> * 4, down_wave = Down::LDS_BYTES + most_tokens * 16 * FT * 4;
+    const unsigned up_wave = Up::LDS_BYTES + 2 * Up::SET_FLOATS * 4, down_wave = Down::LDS_BYTES + most_tokens * 16 * FT * 4;
     const unsigned up_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / up_wave), down_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / down_wave);
     const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), 256);
     hipError_t e = launch_args(up, dim3(groups, rows), dim3(up_waves * 64), up_waves * up_wave + table, s, a);
@@ -682,13 +672,13 @@ hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
 template <typename T, int N2>
 hipError_t launch_columns(const MoeArgs &a, hipStream_t s)
 {
-    if (!a.group) return launch_experts<T, false, N2, 1, false>(a, s);
+    if (!a.group) return launch_experts<T, false, N2, 128, false>(a, s);
     auto folds = [&](auto n) {
         return a.gate_up.w4.zeros ? launch_experts<T, true, N2, decltype(n)::value, true>(a, s) : launch_experts<T, true, N2, decltype(n)::value, false>(a, s);
     };
-    if (a.group % 128 == 0) return folds(std::integral_constant<int, 1>());
-    if (a.group % 64 == 0) return folds(std::integral_constant<int, 2>());
-    return folds(std::integral_constant<int, 4>());
+    if (a.group % 128 == 0) return folds(std::integral_constant<int, 128>());
+    if (a.group % 64 == 0) return folds(std::integral_constant<int, 64>());
+    return folds(std::integral_constant<int, 32>());
 }
 
 template <typename T>

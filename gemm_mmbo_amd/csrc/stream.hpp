@@ -5,19 +5,20 @@
 // Each wavefront of a work-group has the same rows and a run of k of its own; the sums meet in LDS at the end, in the order of the wavefronts.
 //
 // Weights, their scales and columns go through a ring of the wavefront's own in LDS that direct loads fill, DEPTH blocks ahead: no barrier before the sums,
-// no register for what is under way.  Loads have to come as 64 contiguous bytes to four lanes: with a lane to a row, as MFMAs want them, a CU got 11
-// bytes a clock (4096 x 16 x 14336 in 4 bits: 24 us).
+// no register for what is under way.  Loads have to come as whole memory lines: with a lane to a row, as MFMAs want them, a CU got 11 bytes a clock
+// (4096 x 16 x 14336 in 4 bits: 24 us), with 64 bytes to four lanes 20 (13.3 us), though halves of a line were asked for one behind the other.
 //
-// 4-bit weights: a block is 128 places, 64 bytes of a row.  Eight codes become numbers by moving nibbles to where a mantissa ends:
+// 4-bit weights: a block is 128 places, half a line of a row (whole lines took longer: 28672 x 1 x 8192 33 us, with half of them 28).  Eight codes become numbers by moving nibbles to where a mantissa ends:
 //   fp16: the code itself, as a subnormal number (code * 2^-24; MFMAs take those as they are): 7 instructions.
 //   bf16: 128 + code, the largest such number with 4 free bits: 9 instructions.
 // One MFMA against ones sums the columns' elements of a group; zero point (+ 128) times that comes off the group's sums, which then are multiplied by
 // its scale, in fp32.  The sums lose five bits of fp32's 24 to the 128 at most, of which a store to bf16 keeps 8.
-// 16-bit weights: a block is 64 places, 128 bytes of a row.
+// 16-bit weights: a block is 64 places, a line of a row.
 #pragma once
 
 #include <type_traits>
 
+#include "gemm_ring.hpp"
 #include "w4.hpp"
 
 namespace mmbo {
@@ -110,10 +111,11 @@ __device__ inline typename Type<T>::Frag ones()
 }
 
 // 16 bytes a lane from `p` to LDS at lds_addr + 16 * lane; 2 bytes or 1, as a dword, to lds_addr + 4 * lane (lanes that take no part leave theirs as it
-// is).  As ring::direct_load16, but from an address a lane: rows may lie anywhere.
+// is).  As ring::direct_load16, but from an address a lane: rows may lie anywhere.  (The instruction's offset counts for both places.)
+template <int OFFSET = 0>
 __device__ inline void direct_load(const void *p, uint32_t lds_addr)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(p), "s"(lds_addr - OFFSET), "n"(OFFSET) : "memory");
 }
 __device__ inline void direct_load_u16(const void *p, uint32_t lds_addr)
 {
@@ -124,43 +126,77 @@ __device__ inline void direct_load_u8(const void *p, uint32_t lds_addr)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(p), "s"(lds_addr) : "memory");
 }
 
-// Rows of 64 bytes in LDS as direct loads put them: lane l loads chunk (l % 4) ^ (row / 4 % 4) of row l / 4 (of R, then 32 places further).  The exclusive or
-// spreads what is read together over the banks: one chunk of 16 rows, or a dword of each of their four chunks.
-template <int R>
-__device__ inline uint32_t chunk_of_lane(int lane) { return (lane & 3) ^ ((lane >> 2) % R >> 2 & 3); }
-__device__ inline uint32_t chunk_at(uint32_t row, uint32_t chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
-
-// Columns side by side in LDS: 1, 4, 16 or 32.  Columns in PLANES numbers of type T each, which are added.
-template <int N2> constexpr int tiles_of() { return N2 > 16 ? N2 / 16 : 1; }
-
-// Where a lane finds a job's rows of weights in FT tiles of 16, and its columns.  In the place of rows and columns that do not exist: others that do.
-template <typename T, int N2, int FT, int PLANES>
-struct Job {
-    const uint8_t *w[FT];                       // row lane / 4 of codes, or of elements
-    const T *scales[FT];                        // row lane % 16
-    const uint8_t *zeros[FT];
-    const T *x[PLANES][tiles_of<N2>()];         // column lane / 4 % N2 of each tile
-    bool x_here[tiles_of<N2>()];                // .. exists
-};
+// Rows of 128 bytes in LDS as direct loads put them: lane l loads a 16-byte chunk of row l / 8 (of eight, and of the eight behind them with the next load), and the
+// place that is its own takes chunk (l % 8) ^ (row / 2 % 8).  The exclusive or spreads over the banks what is read together: one chunk of 16 rows, or a dword of
+// each of four lanes' chunks.  Rows of 64 bytes: row l / 4, chunk (l % 4) ^ (row / 4 % 4).
+template <int ROW_BYTES>
+__device__ inline uint32_t chunk_of(uint32_t row, int lane) { return ROW_BYTES == 64 ? (lane & 3) ^ (row >> 2 & 3) : (lane & 7) ^ (row >> 1 & 7); }
+template <int ROW_BYTES>
+__device__ inline uint32_t chunk_at(uint32_t row, uint32_t chunk)
+{
+    return ROW_BYTES == 64 ? row * 64 + ((chunk ^ (row >> 2 & 3)) << 4) : row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
+}
 
 // The sums of a wavefront over its share of several jobs: of each job blocks block0 .. block0 + per_job - 1 of k, job after job, and of all these blocks
-// numbers first .. first + count - 1.  enter(job, Job &) says where its operands lie, flush(job, sums) takes the sums of what the wavefront had of it.  Results of columns that do not
-// exist are not defined.  lds: the wavefront's own LDS_BYTES.
-// FOLDS (4-bit weights): times in a block that sums are multiplied by their scale: 1 where groups are whole multiples of 128, 2 of 64, else 4.
-template <typename T, bool W4, int N2, int FT, int PLANES, int FOLDS, bool ZEROS, int DEPTH>
+// numbers first .. first + count - 1.  enter(job, Job &) says where its operands lie, flush(job, sums) takes the sums of what the wavefront had of it.  Results
+// of columns that do not exist are not defined.  lds: the wavefront's own LDS_BYTES.
+// N2: columns side by side, 1, 4, 16 or 32, each in PLANES numbers of type T, which are added.  FT: tiles of 16 rows.
+// FOLD (4-bit weights): places whose sums are multiplied by a scale at once: 128 where groups are whole multiples of that, 64, else 32.
+template <typename T, bool W4, int N2, int FT, int PLANES, int FOLD, bool ZEROS, int DEPTH>
 struct Stream {
+    static_assert(N2 == 1 || N2 == 4 || N2 == 16 || N2 == 32, "");
     typedef typename Type<T>::Frag Frag;
     typedef typename Codes<T>::Masks Masks;
-    typedef stream::Job<T, N2, FT, PLANES> Job;
-    static constexpr int NT = tiles_of<N2>(), BLOCK = W4 ? 128 : 64, STEPS = BLOCK / 32, ROW_BYTES = W4 ? 64 : 128;
-    static constexpr int W_LOADS = ROW_BYTES / 64, W_BYTES = FT * W_LOADS * 1024;
-    static constexpr int X_LANES = N2 < 16 ? STEPS * N2 * 4 : 64, X_LOADS = N2 < 16 ? 1 : STEPS * NT, X_PLANE = N2 < 16 ? STEPS * N2 * 64 : X_LOADS * 1024;
-    static constexpr int X_AT = W_BYTES, S_AT = X_AT + PLANES * X_PLANE, Z_AT = S_AT + (W4 ? FT * 256 : 0), SLOT = Z_AT + (W4 && ZEROS ? FT * 256 : 0);
-    static constexpr int LOADS = FT * W_LOADS + PLANES * X_LOADS + (W4 ? FT * (ZEROS ? 2 : 1) : 0);
+    static constexpr int NT = N2 > 16 ? N2 / 16 : 1, BLOCK = W4 ? 128 : 64, STEPS = BLOCK / 32, ROW_BYTES = W4 ? BLOCK / 2 : 128;
+    static constexpr int FOLDS = W4 ? BLOCK / FOLD : 1;
+    static constexpr int WP = ROW_BYTES / 64, W_TILE = WP * 1024;
+    static constexpr int X_LINES = BLOCK / 64, XP = N2 < 8 ? 1 : N2 / 8, X_LANES = X_LINES * N2 * 8 < 64 ? X_LINES * N2 * 8 : 64,
+                         X_LOADS = (X_LINES * N2 * 8 + 63) / 64, X_PLANE = X_LINES * N2 * 128;
+    static constexpr int S_LOADS = W4 ? (FOLDS + 3) / 4 : 0, S_TILE = FOLDS * 64;
+    static constexpr int X_AT = FT * W_TILE, S_AT = X_AT + PLANES * X_PLANE, Z_AT = S_AT + (W4 ? FT * S_TILE : 0), SLOT = (Z_AT + (W4 && ZEROS ? FT * S_TILE : 0) + 127) / 128 * 128;
+    static constexpr int LOADS = FT * WP + PLANES * X_LOADS + FT * S_LOADS * (ZEROS ? 2 : 1);
     static constexpr int LDS_BYTES = (DEPTH * SLOT + 1023) / 1024 * 1024;
     static_assert((DEPTH - 1) * LOADS < 64, "vmcnt counts to 63");
-    static_assert(N2 == 1 || N2 == 4 || N2 == 16 || N2 == 32, "");
     typedef f32x4 Sums[NT][FT];
+    // A wavefront's sums in LDS: of a tile all columns that there may be.
+    static constexpr int TILE_FLOATS = N2 < 16 ? 16 * N2 : 256, SET_FLOATS = NT * FT * TILE_FLOATS;
+    __device__ static inline void put(float *to, const Sums &acc, int lane)
+    {
+        if (N2 < 16 && lane >= 16) return;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int f = 0; f < FT; ++f) {
+                if constexpr (N2 == 1) to[(c * FT + f) * TILE_FLOATS + lane] = acc[c][f][0];
+                else *reinterpret_cast<f32x4 *>(to + (c * FT + f) * TILE_FLOATS + lane * 4) = acc[c][f];
+            }
+    }
+    // What `waves` wavefronts have of row `row` of tile f and column `col`, added in their order; set: the first one's.
+    __device__ static inline float total(const float *set, uint32_t f, uint32_t row, uint32_t col, uint32_t waves)
+    {
+        const float *at = set + (col / 16 * FT + f) * TILE_FLOATS + (N2 == 1 ? row : ((col >> 2 & 3) * 16 + row) * 4 + (col & 3));
+        float v = at[0];
+        for (uint32_t w = 1; w < waves; ++w) v += at[w * SET_FLOATS];
+        return v;
+    }
+    // Every wavefront of the work-group has put its sums (not __syncthreads(): what is under way stays so).
+    __device__ static inline void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+    // Where a lane finds a job's rows of weights and its columns, from their first place on.  In the place of those that do not exist: others that do.
+    struct Job {
+        const uint8_t *w[FT][WP];               // rows load_row(lane, 0 ..) of a tile: of codes, or of elements
+        const T *scales[FT];                    // row lane % 16
+        const uint8_t *zeros[FT];
+        const T *x[PLANES][XP];                 // columns load_column(lane, 0 ..)
+        bool x_here[XP];                        // .. exist
+    };
+    __device__ static inline uint32_t load_row(int lane, int p) { return ROW_BYTES == 64 ? lane >> 2 : p * 8 + (lane >> 3); }
+    __device__ static inline uint32_t load_column(int lane, int p) { return N2 < 8 ? (lane >> 3) & (N2 - 1) : p * 8 + (lane >> 3); }
+    // of load j: the first place of its line in the block
+    __device__ static inline uint32_t x_line(int lane, int j) { return 64 * (N2 < 8 ? lane / (8 * N2) + j * (8 / N2) : j / XP); }
+    __device__ static inline uint32_t w_chunk(int lane, int p) { return chunk_of<ROW_BYTES>(load_row(lane, p), lane); }
+    __device__ static inline uint32_t x_chunk(int lane, int p) { return chunk_of<128>(load_column(lane, p), lane); }
+    __host__ __device__ static inline uint32_t blocks_of(uint32_t k) { return (k + BLOCK - 1) / BLOCK; }
 
     uint32_t k, group32;                        // places; places of a group / 32
     char *lds;
@@ -168,7 +204,7 @@ struct Stream {
     uint32_t lds_at, block0, per_job;
     // requests
     Job from;
-    uint32_t r_job, r_block, group, rest;       // (group and rest: of the lane's fold)
+    uint32_t r_job, r_block, group[S_LOADS + 1], rest[S_LOADS + 1];                     // (of the lane's folds)
     // products
     Masks masks;
     struct Operands {
@@ -183,7 +219,6 @@ struct Stream {
           per_job(per_job), masks(Codes<T>::masks())
     {
     }
-    __host__ __device__ static inline uint32_t blocks_of(uint32_t k) { return (k + BLOCK - 1) / BLOCK; }
 
     template <typename Enter>
     __device__ inline void enter_job(const Enter &enter)
@@ -191,18 +226,21 @@ struct Stream {
         enter(r_job, from);
         const uint32_t b = block0 + r_block;
 #pragma unroll
-        for (int f = 0; f < FT; ++f) from.w[f] += (uint64_t)b * ROW_BYTES + chunk_of_lane<16>(lane) * 16;
-        const uint32_t place = b * BLOCK + (N2 < 16 ? lane / (4 * N2) * 32 : 0) + chunk_of_lane<(N2 < 16 ? N2 : 16)>(lane) * 8;
+        for (int f = 0; f < FT; ++f)
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            from.x_here[c] = from.x_here[c] && lane < X_LANES;
+            for (int p = 0; p < WP; ++p) from.w[f][p] += (uint64_t)b * ROW_BYTES + w_chunk(lane, p) * 16;
 #pragma unroll
-            for (int q = 0; q < PLANES; ++q) from.x[q][c] += place;
+        for (int p = 0; p < XP; ++p) {
+            // (a load without a lane is none, and would not count: the first column of an eight comes in any case)
+            from.x_here[p] = (from.x_here[p] || lane < 8) && lane < X_LANES;
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q) from.x[q][p] += b * BLOCK + x_chunk(lane, p) * 8 + (N2 < 8 ? x_line(lane, 0) : 0);
         }
-        if constexpr (W4) {
-            const uint32_t at = b * 4 + (lane >> 4) * (4 / FOLDS);
-            group = at / group32;
-            rest = at % group32;
+#pragma unroll
+        for (int j = 0; j < S_LOADS; ++j) {
+            const uint32_t at = b * STEPS + (j * 4 + (lane >> 4)) * (STEPS / FOLDS);
+            group[j] = at / group32;
+            rest[j] = at % group32;
         }
     }
     template <typename Enter>
@@ -214,60 +252,64 @@ struct Stream {
             enter_job(enter);
         }
         const uint32_t to = lds_at + slot * SLOT;
-        if constexpr (W4) {
-            // lane: row lane % 16, fold lane / 16
-            const uint32_t g = min(group, (k - 1) / 32 / group32);
-            if (lane < 16 * FOLDS)
+        // scales: lane's row lane % 16, its folds lane / 16 and every fourth behind that
+#pragma unroll
+        for (int j = 0; j < S_LOADS; ++j) {
+            const uint32_t g = min(group[j], (k - 1) / 32 / group32);
+            if (FOLDS >= 4 || lane < 16 * FOLDS)
 #pragma unroll
                 for (int f = 0; f < FT; ++f) {
-                    direct_load_u16(from.scales[f] + g, to + S_AT + f * 256);
-                    if constexpr (ZEROS) direct_load_u8(from.zeros[f] + g, to + Z_AT + f * 256);
+                    direct_load_u16(from.scales[f] + g, to + S_AT + f * S_TILE + j * 256);
+                    if constexpr (ZEROS) direct_load_u8(from.zeros[f] + g, to + Z_AT + f * S_TILE + j * 256);
                 }
-            group += 4 / group32;
-            rest += 4 % group32;
-            if (rest >= group32) { rest -= group32; ++group; }
+            group[j] += STEPS / group32;
+            rest[j] += STEPS % group32;
+            if (rest[j] >= group32) { rest[j] -= group32; ++group[j]; }
         }
         if ((block0 + r_block) * BLOCK + BLOCK <= k) {
 #pragma unroll
             for (int f = 0; f < FT; ++f)
 #pragma unroll
-                for (int h = 0; h < W_LOADS; ++h) direct_load(from.w[f] + h * 64, to + (f * W_LOADS + h) * 1024);
+                for (int p = 0; p < WP; ++p) direct_load(from.w[f][p], to + f * W_TILE + p * 1024);
 #pragma unroll
             for (int q = 0; q < PLANES; ++q)
-#pragma unroll
-                for (int j = 0; j < X_LOADS; ++j)
-                    if (from.x_here[j % NT]) direct_load(from.x[q][j % NT] + j / NT * 32, to + X_AT + q * X_PLANE + j * 1024);
+                ring::static_for<X_LOADS>([&](auto J) {
+                    constexpr int j = decltype(J)::value;
+                    if (from.x_here[j % XP]) direct_load<(N2 < 8 ? j * (8 / N2) : j / XP) * 128>(from.x[q][j % XP], to + X_AT + q * X_PLANE + j * 1024);
+                });
         } else {
-            // The last block of a k that is not a whole number of them: chunks that are there as ever, the others through registers.  Counts of
-            // what is under way no longer hold then, so nothing is, for once.
+            // The last block of a k that is not a whole number of them, through registers.  Counts of what is under way no longer hold then, so nothing is,
+            // for once.
             const int64_t left = (int64_t)k - (block0 + r_block) * BLOCK;
             char *const slot_at = lds + slot * SLOT;
 #pragma unroll
             for (int f = 0; f < FT; ++f)
 #pragma unroll
-                for (int h = 0; h < W_LOADS; ++h) {
-                    const int64_t here = left - h * 32 - chunk_of_lane<16>(lane) * (W4 ? 32 : 8);
-                    u32x4 *const at = reinterpret_cast<u32x4 *>(slot_at + (f * W_LOADS + h) * 1024 + lane * 16);
-                    if constexpr (W4) *at = here >= 32 ? *reinterpret_cast<const u32x4_any *>(from.w[f]) : load32_codes(from.w[f], here);
-                    else *at = load8(reinterpret_cast<const T *>(from.w[f] + h * 64), here);
+                for (int p = 0; p < WP; ++p) {
+                    const int64_t here = left - w_chunk(lane, p) * (W4 ? 32 : 8);
+                    u32x4 *const at = reinterpret_cast<u32x4 *>(slot_at + f * W_TILE + p * 1024 + lane * 16);
+                    if constexpr (W4) *at = here >= 32 ? *reinterpret_cast<const u32x4_any *>(from.w[f][p]) : load32_codes(from.w[f][p], here);
+                    else *at = load8(reinterpret_cast<const T *>(from.w[f][p]), here);
                 }
 #pragma unroll
             for (int q = 0; q < PLANES; ++q)
 #pragma unroll
                 for (int j = 0; j < X_LOADS; ++j)
-                    if (from.x_here[j % NT]) {
-                        const int64_t here = left - (N2 < 16 ? lane / (4 * N2) : j / NT) * 32 - chunk_of_lane<(N2 < 16 ? N2 : 16)>(lane) * 8;
-                        *reinterpret_cast<u32x4 *>(slot_at + X_AT + q * X_PLANE + j * 1024 + lane * 16) = load8(from.x[q][j % NT] + j / NT * 32, here);
+                    if (from.x_here[j % XP]) {
+                        const int64_t here = left - x_line(lane, j) - x_chunk(lane, j % XP) * 8;
+                        *reinterpret_cast<u32x4 *>(slot_at + X_AT + q * X_PLANE + j * 1024 + lane * 16) = load8(from.x[q][j % XP] + x_line(0, j), here);
                     }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         ++r_block;
 #pragma unroll
-        for (int f = 0; f < FT; ++f) from.w[f] += ROW_BYTES;
+        for (int f = 0; f < FT; ++f)
+#pragma unroll
+            for (int p = 0; p < WP; ++p) from.w[f][p] += ROW_BYTES;
 #pragma unroll
         for (int q = 0; q < PLANES; ++q)
 #pragma unroll
-            for (int c = 0; c < NT; ++c) from.x[q][c] += BLOCK;
+            for (int p = 0; p < XP; ++p) from.x[q][p] += BLOCK;
     }
 
     __device__ inline void read(uint32_t slot)
@@ -280,20 +322,21 @@ struct Stream {
             for (int i = 0; i < STEPS; ++i)
 #pragma unroll
                 for (int c = 0; c < NT; ++c)
-                    o.x[q][i][c] = frag_of<T>(*reinterpret_cast<const u32x4 *>(at + X_AT + q * X_PLANE + i * N2 * 64 + chunk_at((lane & (N2 < 16 ? N2 - 1 : 15)) + c * 16, quarter)));
+                    o.x[q][i][c] = frag_of<T>(*reinterpret_cast<const u32x4 *>(at + X_AT + q * X_PLANE + i / 2 * N2 * 128 +
+                                                                               chunk_at<128>((lane & (N2 < 16 ? N2 - 1 : 15)) + c * 16, i % 2 * 4 + quarter)));
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
             if constexpr (W4) {
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) o.codes[i][f] = *reinterpret_cast<const uint32_t *>(at + f * 1024 + chunk_at(row, i) + quarter * 4);
+                for (int i = 0; i < STEPS; ++i) o.codes[i][f] = *reinterpret_cast<const uint32_t *>(at + f * W_TILE + chunk_at<ROW_BYTES>(row, i) + quarter * 4);
 #pragma unroll
                 for (int q = 0; q < FOLDS; ++q) {
-                    o.scales[q][f] = *reinterpret_cast<const uint32_t *>(at + S_AT + f * 256 + (q * 16 + row) * 4);
-                    if constexpr (ZEROS) o.zeros[q][f] = *reinterpret_cast<const uint32_t *>(at + Z_AT + f * 256 + (q * 16 + row) * 4);
+                    o.scales[q][f] = *reinterpret_cast<const uint32_t *>(at + S_AT + f * S_TILE + (q * 16 + row) * 4);
+                    if constexpr (ZEROS) o.zeros[q][f] = *reinterpret_cast<const uint32_t *>(at + Z_AT + f * S_TILE + (q * 16 + row) * 4);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) o.w[i][f] = *reinterpret_cast<const u32x4 *>(at + (f * STEPS + i) * 1024 + chunk_at(row, quarter));
+                for (int i = 0; i < STEPS; ++i) o.w[i][f] = *reinterpret_cast<const u32x4 *>(at + f * W_TILE + chunk_at<128>(row, i * 4 + quarter));
             }
         }
     }
@@ -309,7 +352,7 @@ struct Stream {
 #pragma unroll
                 for (int c = 0; c < NT; ++c) sums[c] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int i = q * (4 / FOLDS); i < (q + 1) * (4 / FOLDS); ++i) {
+                for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i) {
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -395,75 +438,61 @@ struct Stream {
     }
 };
 
-// Tiles of 16 x 16 sums of several wavefronts -> their sum: wavefront after wavefront, in that order.  lds: waves * TILES * 256 floats.  Gives element `at` of
-// TILES * 256: column at / 16 % 16, row at % 16 of tile at / 256.
-template <int TILES>
-__device__ inline void put_sums(float *lds, const f32x4 (&acc)[TILES], int wave, int lane)
-{
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) *reinterpret_cast<f32x4 *>(lds + (wave * TILES + t) * 256 + lane * 4) = acc[t];
-}
-template <int TILES>
-__device__ inline float sum_of(const float *lds, uint32_t at, int waves)
-{
-    const uint32_t row = at & 15, col = at >> 4 & 15, tile = at >> 8;
-    const uint32_t place = tile * 256 + ((col >> 2) * 16 + row) * 4 + (col & 3);
-    float v = lds[place];
-    for (int w = 1; w < waves; ++w) v += lds[w * TILES * 256 + place];
-    return v;
-}
-
 }  // namespace stream
 
-// A work-group: 16 * FT rows of W, up to N2 columns of B; its wavefronts share k, a run of blocks each.
-template <typename T, int N2, int FT, int FOLDS, bool ZEROS, int DEPTH>
+// A unit of work: 16 * FT rows of W, N2 columns of B, k shared by the wavefronts.  A work-group takes a run of units, one behind the other without a pause in its
+// loads: the wavefronts meet once a unit, over two sets of sums in turn.
+template <typename T, int N2, int FT, int FOLD, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(512)
 gemm_w4_stream_kernel(const GemmW4Args a)
 {
     using namespace stream;
-    typedef Stream<T, true, N2, FT, 1, FOLDS, ZEROS, DEPTH> S;
-    constexpr int NT = S::NT, TILES = NT * FT;
+    typedef Stream<T, true, N2, FT, 1, FOLD, ZEROS, DEPTH> S;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint64_t row0 = (uint64_t)blockIdx.x * 16 * FT;
-    auto enter = [&](uint32_t, typename S::Job &j) {
+    const uint32_t all = (a.m + 16 * FT - 1) / (16 * FT), col0 = blockIdx.y * N2;
+    const uint32_t unit0 = (uint32_t)((uint64_t)all * blockIdx.x / gridDim.x), units = (uint32_t)((uint64_t)all * (blockIdx.x + 1) / gridDim.x) - unit0;
+    float *const sums = reinterpret_cast<float *>(lds + waves * S::LDS_BYTES);           // [set][wavefront][..]
+    auto enter = [&](uint32_t u, typename S::Job &j) {
+        const uint32_t row0 = (unit0 + u) * 16 * FT;
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
-            const uint64_t i = min(row0 + f * 16 + (lane & 15), (uint64_t)a.m - 1);         // (rows past the edge repeat the last one)
-            j.w[f] = a.w.q + min(row0 + f * 16 + (lane >> 2), (uint64_t)a.m - 1) * a.w.ldq;
+            const uint64_t i = min(row0 + f * 16 + (lane & 15), a.m - 1);               // (rows past the edge repeat the last one)
+#pragma unroll
+            for (int q = 0; q < S::WP; ++q) j.w[f][q] = a.w.q + (uint64_t)min(row0 + f * 16 + S::load_row(lane, q), a.m - 1) * a.w.ldq;
             j.scales[f] = static_cast<const T *>(a.w.scales) + i * a.w.lds;
-            j.zeros[f] = a.w.zeros + i * a.w.ldz;
+            j.zeros[f] = ZEROS ? a.w.zeros + i * a.w.ldz : nullptr;
         }
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            const uint32_t col = (uint32_t)(lane >> 2) % N2 % 16 + c * 16;
-            j.x[0][c] = static_cast<const T *>(a.B) + min(col, a.n - 1) * a.ldb;
-            j.x_here[c] = col < a.n;
+        for (int q = 0; q < S::XP; ++q) {
+            const uint32_t col = col0 + S::load_column(lane, q);
+            j.x[0][q] = static_cast<const T *>(a.B) + min(col, a.n - 1) * a.ldb;
+            j.x_here[q] = col < a.n;
         }
     };
-    f32x4 total[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) total[t] = f32x4{0, 0, 0, 0};
-    auto flush = [&](uint32_t, const typename S::Sums &acc) {
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) total[t] = acc[t / FT][t % FT];
+    auto flush = [&](uint32_t u, const typename S::Sums &acc) {
+        float *const set = sums + (u & 1) * waves * S::SET_FLOATS;
+        S::put(set + wave * S::SET_FLOATS, acc, lane);
+        S::meet();
+        const uint32_t row0 = (unit0 + u) * 16 * FT;
+        for (uint32_t at = threadIdx.x; at < 16 * FT * N2; at += blockDim.x) {
+            const uint32_t f = at / 16 % FT, col = at / (16 * FT), i = row0 + f * 16 + (at & 15), j = col0 + col;
+            if (i >= a.m || j >= a.n) continue;
+            T *c = static_cast<T *>(a.C) + i + j * a.ldc;
+            float v = a.alpha * S::total(set, f, at & 15, col, waves);
+            if (a.beta != 0.0f) v = __builtin_fmaf(a.beta, (float)*c, v);
+            *c = (T)v;
+        }
     };
-    const uint32_t blocks = S::blocks_of(a.k), each = blocks / waves, more = blocks % waves, count = each + (wave < more);
-    S s(a.k, a.group / kW4Group, wave * each + min(wave, more), count, lds + wave * S::LDS_BYTES, lane);
-    s.run(0, count, enter, flush);
-    __syncthreads();                                                                    // (the sums lie where the rings were)
-    float *sums = reinterpret_cast<float *>(lds);
-    put_sums<TILES>(sums, total, wave, lane);
-    __syncthreads();
-    for (uint32_t at = threadIdx.x; at < TILES * 256; at += blockDim.x) {
-        const uint32_t tile = at >> 8;
-        const uint64_t i = row0 + tile % FT * 16 + (at & 15), j = tile / FT * 16 + (at >> 4 & 15);
-        if (i >= a.m || j >= a.n) continue;
-        T *c = static_cast<T *>(a.C) + i + j * a.ldc;
-        float v = a.alpha * sum_of<TILES>(sums, at, waves);
-        if (a.beta != 0.0f) v = __builtin_fmaf(a.beta, (float)*c, v);
-        *c = (T)v;
+    const uint32_t blocks = S::blocks_of(a.k), each = blocks / waves, more = blocks % waves, mine = each + (wave < more);
+    S s(a.k, a.group / kW4Group, wave * each + min(wave, more), mine, lds + wave * S::LDS_BYTES, lane);
+    if (mine != 0) {
+        s.run(0, units * mine, enter, flush);
+    } else {                                                                            // k is 0: nothing to add
+        typename S::Sums none;
+        S::clear(none);
+        for (uint32_t u = 0; u < units; ++u) flush(u, none);
     }
 }
 

@@ -5,7 +5,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "stream.hpp"
+#include "w4_tile.hpp"
 
 namespace mmbo {
 namespace {
@@ -189,61 +189,118 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
 
 constexpr int kStreamWaves = 8;
 
-template <typename T, int N2, int FT, int FOLDS, bool ZEROS>
+
+template <typename T, int N2, int FT, int FOLD, bool ZEROS>
 hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
 {
     // Blocks under way in a ring.  Work-groups beside each other on a CU hide what a deeper ring would, and need the LDS: 28672 x 1 x 8192 29.4 us
-    // with rings of 3, 28.4 of 2, 33.7 of 3 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 of 2, 13.6 of 3, 14.5 of 4.
+    // with rings of 3, 33.7 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 with rings of 2, 13.6 of 3, 14.5 of 4.
     constexpr int DEPTH = N2 == 1 ? 3 : 2;
-    typedef stream::Stream<T, true, N2, FT, 1, FOLDS, ZEROS, DEPTH> S;
-    constexpr int kWaveBytes = std::max(S::LDS_BYTES, stream::tiles_of<N2>() * FT * 1024);
-    constexpr int kMost = std::min(kStreamWaves, 160 * 1024 / kWaveBytes);
+    typedef stream::Stream<T, true, N2, FT, 1, FOLD, ZEROS, DEPTH> S;
+    constexpr int kWaveBytes = S::LDS_BYTES + 2 * S::SET_FLOATS * 4, kMost = std::min(kStreamWaves, 160 * 1024 / kWaveBytes);
     static std::atomic<bool> set[64];
-    auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLDS, ZEROS, DEPTH>;
+    auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLD, ZEROS, DEPTH>;
     if (hipError_t e = allow_lds(kernel, set)) return e;
     const int waves = (int)std::max<uint32_t>(std::min<uint32_t>(S::blocks_of(a.k), kMost), 1);
-    return launch_args(kernel, dim3((unsigned)ceil_div(a.m, 16 * FT)), dim3(waves * 64), waves * kWaveBytes, s, a);
+    // as many work-groups as the CUs hold at a time, two of eight wavefronts each at most (128256 x 1 x 4096: one 68, two 58, three 58 us)
+    const unsigned columns = (unsigned)ceil_div(a.n, N2), held = 256 * std::min<unsigned>(160 * 1024 / (waves * kWaveBytes), 2 * kStreamWaves / waves);
+    const unsigned groups = (unsigned)std::min<size_t>(ceil_div(a.m, 16 * FT), std::max(held / columns, 1u));
+    return launch_args(kernel, dim3(groups, columns), dim3(waves * 64), waves * kWaveBytes, s, a);
 }
 
-template <typename T, int N2, int FT, int FOLDS>
+template <typename T, int N2, int FT, int FOLD>
 hipError_t launch_stream_folds(const GemmW4Args &a, hipStream_t s)
 {
-    return a.w.zeros ? launch_stream_kernel<T, N2, FT, FOLDS, true>(a, s) : launch_stream_kernel<T, N2, FT, FOLDS, false>(a, s);
+    return a.w.zeros ? launch_stream_kernel<T, N2, FT, FOLD, true>(a, s) : launch_stream_kernel<T, N2, FT, FOLD, false>(a, s);
 }
 
 template <typename T, int N2, int FT>
 hipError_t launch_stream_tile(const GemmW4Args &a, hipStream_t s)
 {
-    if (a.group % 128 == 0) return launch_stream_folds<T, N2, FT, 1>(a, s);
-    if (a.group % 64 == 0) return launch_stream_folds<T, N2, FT, 2>(a, s);
-    return launch_stream_folds<T, N2, FT, 4>(a, s);
+    if (a.group % 128 == 0) return launch_stream_folds<T, N2, FT, 128>(a, s);
+    if (a.group % 64 == 0) return launch_stream_folds<T, N2, FT, 64>(a, s);
+    return launch_stream_folds<T, N2, FT, 32>(a, s);
 }
 
 template <typename T, int N2>
 hipError_t launch_stream_columns(const GemmW4Args &a, hipStream_t s)
 {
     // Two tiles of rows a work-group where that still is a work-group for each of 256 CUs: the columns, which every work-group reads, are then read half as
-    // often.  8192 x 16 x 8192 11.3 us beside 14.5, 128256 x 1 x 4096 53.9 beside 61.3; 4096 x 16 x 14336 16.2 beside 13.3.
+    // often.  8192 x 16 x 8192 12.2 us beside 12.4, 14336 x 4 x 4096 9.4 beside 9.8, 128256 x 1 x 4096 58 beside 63; 4096 x 16 x 14336 16.7 beside 13.1.
     return a.m >= 256 * 32 ? launch_stream_tile<T, N2, 2>(a, s) : launch_stream_tile<T, N2, 1>(a, s);
 }
 
-template <typename T>
-hipError_t launch_stream(const GemmW4Args &all, hipStream_t s)
+template <typename T, int WM, int NC, int FOLDS, bool ZEROS>
+hipError_t launch_tile_kernel(const GemmW4Args &a, hipStream_t s)
 {
-    constexpr uint32_t kRows = 1u << 26;         // of one launch: a grid has less than 2^32 threads
+    typedef tile::Config<T, WM, NC, FOLDS, ZEROS, 3> C;
+    if constexpr (!C::FITS) {                    // (eight wavefronts with four scales and zero points a slot)
+        return launch_tile_kernel<T, WM / 2, NC, FOLDS, ZEROS>(a, s);
+    } else {
+    static std::atomic<bool> set[64];
+    auto kernel = gemm_w4_tile_kernel<T, WM, NC, FOLDS, ZEROS, 3>;
+    if (hipError_t e = allow_lds(kernel, set)) return e;
+    return launch_args(kernel, dim3((unsigned)(ceil_div(a.m, C::ROWS) * ceil_div(a.n, C::COLUMNS))), dim3(C::THREADS), C::LDS_BYTES, s, a);
+    }
+}
+
+template <typename T, int WM, int NC>
+hipError_t launch_tile(const GemmW4Args &a, hipStream_t s)
+{
+    auto folds = [&](auto n) {
+        return a.w.zeros ? launch_tile_kernel<T, WM, NC, decltype(n)::value, true>(a, s) : launch_tile_kernel<T, WM, NC, decltype(n)::value, false>(a, s);
+    };
+    if (a.group % 128 == 0) return folds(std::integral_constant<int, 1>());
+    if (a.group % 64 == 0) return folds(std::integral_constant<int, 2>());
+    return folds(std::integral_constant<int, 4>());
+}
+
+// More than 32 columns: what a call takes by each kernel, in us, from rounds of work-groups over the 256 CUs.  Measured, fp16 and bf16, group 128:
+//   stream, 32 x 32 (or 16 x 32): what a work-group pulls at some 47 bytes a ns    128 x 4096 x 4096 17.3, 256 30-32, 512 57-61; 64 x 8192 x 8192 29
+//   tile of 64 x 64, two a CU: 1.1 us a slot of 128 places, 1.4 for a CU with two   256 x 8192 x 4096 45, 512 x 4096 x 4096 45, 1024 87
+//   tile of 256 x 128: 2.1 us a slot                                               512 x 4096 x 4096 64, 1024 66, 2048 x 8192 x 4096 136 and 146
+enum class Kernel { kStream16, kStream32, kTile64, kTile256 };
+Kernel kernel_for(size_t m, size_t n, size_t k)
+{
+    const double slots = (double)ceil_div(k, 128);
+    const size_t tiles32 = ceil_div(m, 32) * ceil_div(n, 32), tiles16 = ceil_div(m, 16) * ceil_div(n, 32), tiles64 = ceil_div(m, 64) * ceil_div(n, 64),
+                 tiles256 = ceil_div(m, 256) * ceil_div(n, 128);
+    const double us[4] = {(double)ceil_div(tiles16, 256) * (double)k * 72 / 47e3, (double)ceil_div(tiles32, 256) * (double)k * 80 / 47e3,
+                          (tiles64 <= 256 ? 1.1 : 1.4 * (double)ceil_div(tiles64, 512)) * slots, 2.1 * (double)ceil_div(tiles256, 256) * slots};
+    return (Kernel)(std::min_element(us, us + 4) - us);
+}
+
+template <typename T>
+hipError_t launch_columns(const GemmW4Args &a, hipStream_t s)
+{
+    if (a.n == 1) return launch_stream_columns<T, 1>(a, s);
+    if (a.n <= 4) return launch_stream_columns<T, 4>(a, s);
+    if (a.n <= 16) return launch_stream_columns<T, 16>(a, s);
+    if (a.n <= 32) return launch_stream_columns<T, 32>(a, s);
+    switch (kernel_for(a.m, a.n, a.k)) {
+        case Kernel::kStream16: return launch_stream_tile<T, 32, 1>(a, s);
+        case Kernel::kStream32: return launch_stream_tile<T, 32, 2>(a, s);
+        case Kernel::kTile64: return launch_tile<T, 2, 4>(a, s);
+        default: return launch_tile<T, 8, 8>(a, s);
+    }
+}
+
+template <typename T>
+hipError_t launch_gemm(const GemmW4Args &all, hipStream_t s)
+{
+    // what one launch may be: a grid has less than 2^32 threads
+    constexpr uint64_t kRows = 1u << 22, kColumns = 1u << 16;
     for (uint64_t i = 0; i < all.m; i += kRows)
-        for (uint64_t j = 0; j < all.n; j += 32) {
+        for (uint64_t j = 0; j < all.n; j += kColumns) {
             GemmW4Args a = all;
-            a.m = (uint32_t)std::min<uint64_t>(all.m - i, kRows);
-            a.n = (uint32_t)std::min<uint64_t>(all.n - j, 32);
+            a.m = (uint32_t)std::min(all.m - i, kRows);
+            a.n = (uint32_t)std::min(all.n - j, kColumns);
             a.w.q += i * a.w.ldq;
             a.w.scales = static_cast<const T *>(a.w.scales) + i * a.w.lds;
             if (a.w.zeros) a.w.zeros += i * a.w.ldz;
             a.B = static_cast<const T *>(all.B) + j * all.ldb;
             a.C = static_cast<T *>(all.C) + i + j * all.ldc;
-            const hipError_t e = a.n == 1 ? launch_stream_columns<T, 1>(a, s) : a.n <= 4 ? launch_stream_columns<T, 4>(a, s)
-                               : a.n <= 16 ? launch_stream_columns<T, 16>(a, s) : launch_stream_columns<T, 32>(a, s);
-            if (e != hipSuccess) return e;
+            if (hipError_t e = launch_columns<T>(a, s)) return e;
         }
     return hipSuccess;
 }
@@ -269,7 +326,26 @@ int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const vo
     const GemmW4Args a{matrix_of(Q, ldq, scales, lds, zeros, ldz), B, C, *static_cast<const float *>(alpha), *static_cast<const float *>(beta),
                        (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)group, ldb, ldc};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return status_of(dtype == MMBO_F16 ? launch_stream<half_t>(a, s) : launch_stream<bf16_t>(a, s));
+    return status_of(dtype == MMBO_F16 ? launch_gemm<half_t>(a, s) : launch_gemm<bf16_t>(a, s));
+}
+
+// Not part of the interface: mmbo_gemm_w4 for packed operands by a given kernel -- 0, 1: 16 or 32 rows of 32 columns on the stream, 2, 3: tiles of 64 x 64 and
+// 256 x 128 -- whatever the pick is: the tests reach each of them through it.
+int mmbo_internal_gemm_w4(int kernel, int dtype, size_t m, size_t n, size_t k, size_t group, const void *Q, const void *scales, const unsigned char *zeros,
+                          const void *B, void *C, void *stream)
+{
+    if (!w4_dtype(dtype)) return MMBO_ERR_INVALID_DTYPE;
+    if (kernel < 0 || kernel > 3) return MMBO_ERR_INVALID_CONFIG;
+    const size_t ldq = (k + 1) / 2 * 2, groups = ceil_div(k, std::max<size_t>(group, 1));
+    if (int rc = check_weight(m, k, group, ldq, groups, zeros, groups)) return rc;
+    if (m == 0 || n == 0 || k == 0 || m > 1 << 22 || n > 1 << 16) return MMBO_ERR_INVALID_SIZE;
+    const GemmW4Args a{matrix_of(Q, ldq, scales, groups, zeros, groups), B, C, 1.0f, 0.0f, (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)group, k, m};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto run = [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return kernel == 0 ? launch_stream_tile<T, 32, 1>(a, s) : kernel == 1 ? launch_stream_tile<T, 32, 2>(a, s) : kernel == 2 ? launch_tile<T, 2, 4>(a, s) : launch_tile<T, 8, 8>(a, s);
+    };
+    return status_of(dtype == MMBO_F16 ? run((half_t *)nullptr) : run((bf16_t *)nullptr));
 }
 
 int mmbo_w4_quantize(int w_dtype, int dtype, size_t m, size_t k, size_t group, const void *W, size_t ldw, void *Q, size_t ldq,

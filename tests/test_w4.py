@@ -121,6 +121,25 @@ def test_products_with_zeros_scalars_and_rows_inside_larger_arrays(dtype, n, pad
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_every_kernel_for_many_columns(dtype, kernel, group):
+    """Each of the kernels that a call with more than 32 columns may be given, on sizes that the pick gives to others too."""
+    f = api.lib().mmbo_internal_gemm_w4
+    f.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_size_t] * 4 + [ctypes.c_void_p] * 6
+    for m, n, k, zeros in ((300, 150, 384, True), (256, 128, 1024, False), (17, 33, 95, True), (70, 260, 640, True), (513, 40, 1003, False), (64, 64, 32, True)):
+        w, b, c = _problem(dtype, m, n, k, group, zeros)
+        q, s, z = w.q.cuda(), w.scales.cuda(), w.zeros.cuda() if zeros else None
+        db, dc = b.cuda(), c.cuda()
+        torch.cuda.synchronize()
+        assert f(kernel, dtype, m, n, k, group, q.data_ptr(), s.data_ptr(), z.data_ptr() if zeros else None, db.data_ptr(), dc.data_ptr(), None) == 0
+        torch.cuda.synchronize()
+        exact, bound = R.gemm(dtype, w, b, 1.0, 0.0, c)
+        _close(dc.cpu(), exact, bound, f"{m}x{n}x{k}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
 def test_no_k_gives_beta_c(dtype):
     for beta in (0.0, 0.5):
         w, b, c = _problem(dtype, 20, 3, 0, 32, beta=beta, pad=1)                # (a leading dimension is 1 at least)
