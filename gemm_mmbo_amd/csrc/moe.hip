@@ -369,6 +369,7 @@ __device__ inline Table stage_table(const MoeArgs &a, uint32_t row, char *lds)
     return table_at(lds, most_pairs, a.most_jobs);
 }
 
+constexpr uint32_t kSelfSelect = 4;             // tokens that are selected by the work-groups of the first product: a launch less
 constexpr int kMoeWaves = 8;                    // or as many as fit the LDS
 constexpr unsigned kLds = 160 * 1024;
 
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
     float *const sums = reinterpret_cast<float *>(lds + waves * S::LDS_BYTES);           // [set][wavefront][tile][..]
     char *const table_lds = reinterpret_cast<char *>(sums + 2 * waves * S::SET_FLOATS);
     Table table;
-    if constexpr (N2 < 16) {
+    if (a.tokens <= kSelfSelect) {
         // A few tokens are selected by every work-group for itself, in less than another launch takes; one of them leaves the table to the next kernel.
         const uint32_t most_pairs = a.tokens * a.top_k;
         table = table_at(table_lds, most_pairs, a.most_jobs);
@@ -587,11 +588,17 @@ int check_layer(const mmbo_moe_layer *l)
 size_t lines(size_t n) { return (n + 127) / 128 * 128; }
 
 // Columns side by side in a stream for so many tokens, and the most jobs that a row of them can make: every job but an expert's last is full.
-uint32_t columns_of(uint32_t tokens) { return tokens == 1 ? 1 : tokens <= 4 ? 4 : 16; }
+// Sixteen take their places in LDS and their loads whether they are there or not; with two pairs to an expert on average one in twenty experts has more than four and
+// is read twice.  (8 tokens, 8 of 64 experts of 2048 x 1024 in 4 bits: 64 us in fours, 71 in sixteens)
+uint32_t columns_of(const mmbo_moe_layer &l, size_t tokens)
+{
+    if (tokens == 1) return 1;
+    return tokens <= 4 || std::min<size_t>(tokens, kTokens) * l.top_k <= 2 * l.experts ? 4 : 16;
+}
 uint32_t most_jobs_of(const mmbo_moe_layer &l, size_t tokens)
 {
     const uint32_t pairs = std::min<uint32_t>((uint32_t)tokens, kTokens) * (uint32_t)l.top_k;
-    return std::min<uint32_t>(pairs, (uint32_t)l.experts + pairs / columns_of((uint32_t)tokens));
+    return std::min<uint32_t>(pairs, (uint32_t)l.experts + pairs / columns_of(l, tokens));
 }
 
 // Work-groups that share a tile of y: as many as make one for each of 256 CUs, up to eight.
@@ -651,7 +658,7 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
 template <typename T, bool W4, int N2, int FOLD, bool ZEROS>
 hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
 {
-    constexpr int UP_DEPTH = N2 < 16 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
+    constexpr int UP_DEPTH = N2 < 16 && !W4 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
     typedef stream::Stream<T, W4, N2, 2, 1, FOLD, ZEROS, UP_DEPTH> Up;
     typedef stream::Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> Down;
     const uint32_t rows = (uint32_t)ceil_div(a.tokens, kTokens), most_tokens = std::min(a.tokens, kTokens);
@@ -663,8 +670,9 @@ hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
     if (hipError_t e = allow_lds(down, set[1])) return e;
     const unsigned up_wave = Up::LDS_BYTES + 2 * Up::SET_FLOATS * 4, down_wave = Down::LDS_BYTES + most_tokens * 16 * FT * 4;
     const unsigned up_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / up_wave), down_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / down_wave);
-    const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), 256);
-    hipError_t e = launch_args(up, dim3(groups, rows), dim3(up_waves * 64), up_waves * up_wave + table, s, a);
+    const unsigned up_lds = up_waves * up_wave + table, held = 256 * std::min<unsigned>(kLds / up_lds, 2);
+    const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), held);
+    hipError_t e = launch_args(up, dim3(groups, rows), dim3(up_waves * 64), up_lds, s, a);
     if (e != hipSuccess) return e;
     return launch_args(down, dim3(a.down_tiles, rows, a.sharers), dim3(down_waves * 64), down_waves * down_wave + table, s, a);
 }
@@ -688,7 +696,7 @@ hipError_t run(const MoeArgs &a, bool router32, hipStream_t s)
     hipError_t e = router32 ? launch_args(moe_logits_kernel<T, float>, logits, dim3(256), 0, s, a)
                             : launch_args(moe_logits_kernel<T, T>, logits, dim3(256), 0, s, a);
     if (e != hipSuccess) return e;
-    if (a.columns >= 16) {
+    if (a.tokens > kSelfSelect) {
         const uint32_t most_tokens = std::min(a.tokens, kTokens);
         e = launch_args(moe_select_kernel, dim3((unsigned)ceil_div(most_tokens, kSelectTokens), (unsigned)ceil_div(a.tokens, kTokens)), dim3(kSelectTokens * 64),
                         select_bytes(most_tokens * a.top_k, a.experts), s, a);
@@ -744,7 +752,7 @@ int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, cons
     a.sharers = sharers_of(l, tokens);
     a.ids = ids;
     a.weights = weights;
-    a.columns = columns_of((uint32_t)tokens);
+    a.columns = columns_of(l, tokens);
     a.most_jobs = most_jobs_of(l, tokens);
     a.tokens = (uint32_t)tokens; a.hidden = (uint32_t)l.hidden; a.inner = (uint32_t)l.inner; a.experts = (uint32_t)l.experts;
     a.top_k = (uint32_t)l.top_k; a.group = (uint32_t)l.group;
