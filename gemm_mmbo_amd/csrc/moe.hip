@@ -656,37 +656,54 @@ hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
 }
 
 template <typename T, bool W4, int N2, int FOLD, bool ZEROS>
+hipError_t launch_gate_up(const MoeArgs &a, hipStream_t s)
+{
+    constexpr int DEPTH = N2 < 16 && !W4 ? 3 : 2;
+    typedef stream::Stream<T, W4, N2, 2, 1, FOLD, ZEROS, DEPTH> S;
+    static std::atomic<bool> set[64];
+    auto kernel = moe_gate_up_kernel<T, W4, N2, FOLD, ZEROS, DEPTH>;
+    if (hipError_t e = allow_lds(kernel, set)) return e;
+    const unsigned table = table_bytes(std::min(a.tokens, kTokens) * a.top_k, a.most_jobs), wave = S::LDS_BYTES + 2 * S::SET_FLOATS * 4;
+    const unsigned waves = std::min<unsigned>(kMoeWaves, (kLds - table) / wave), bytes = waves * wave + table, held = 256 * std::min<unsigned>(kLds / bytes, 2);
+    const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), held);
+    return launch_args(kernel, dim3(groups, (unsigned)ceil_div(a.tokens, kTokens)), dim3(waves * 64), bytes, s, a);
+}
+
+template <typename T, bool W4, int N2, int FOLD, bool ZEROS>
+hipError_t launch_down(const MoeArgs &a, hipStream_t s)
+{
+    constexpr int DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
+    typedef stream::Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> S;
+    static std::atomic<bool> set[64];
+    auto kernel = moe_down_kernel<T, W4, N2, FT, FOLD, ZEROS, DEPTH>;
+    if (hipError_t e = allow_lds(kernel, set)) return e;
+    const uint32_t most_tokens = std::min(a.tokens, kTokens);
+    const unsigned table = table_bytes(most_tokens * a.top_k, a.most_jobs), wave = S::LDS_BYTES + most_tokens * 16 * FT * 4;
+    const unsigned waves = std::min<unsigned>(kMoeWaves, (kLds - table) / wave);
+    return launch_args(kernel, dim3(a.down_tiles, (unsigned)ceil_div(a.tokens, kTokens), a.sharers), dim3(waves * 64), waves * wave + table, s, a);
+}
+
+template <typename T, bool W4, int N2, int FOLD>
 hipError_t launch_experts(const MoeArgs &a, hipStream_t s)
 {
-    constexpr int UP_DEPTH = N2 < 16 && !W4 ? 3 : 2, DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
-    typedef stream::Stream<T, W4, N2, 2, 1, FOLD, ZEROS, UP_DEPTH> Up;
-    typedef stream::Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> Down;
-    const uint32_t rows = (uint32_t)ceil_div(a.tokens, kTokens), most_tokens = std::min(a.tokens, kTokens);
-    const unsigned table = table_bytes(most_tokens * a.top_k, a.most_jobs);
-    static std::atomic<bool> set[2][64];
-    auto up = moe_gate_up_kernel<T, W4, N2, FOLD, ZEROS, UP_DEPTH>;
-    auto down = moe_down_kernel<T, W4, N2, FT, FOLD, ZEROS, DEPTH>;
-    if (hipError_t e = allow_lds(up, set[0])) return e;
-    if (hipError_t e = allow_lds(down, set[1])) return e;
-    const unsigned up_wave = Up::LDS_BYTES + 2 * Up::SET_FLOATS * 4, down_wave = Down::LDS_BYTES + most_tokens * 16 * FT * 4;
-    const unsigned up_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / up_wave), down_waves = std::min<unsigned>(kMoeWaves, (kLds - table) / down_wave);
-    const unsigned up_lds = up_waves * up_wave + table, held = 256 * std::min<unsigned>(kLds / up_lds, 2);
-    const unsigned groups = (unsigned)std::min<size_t>(a.most_jobs * ceil_div(a.inner, 16), held);
-    hipError_t e = launch_args(up, dim3(groups, rows), dim3(up_waves * 64), up_lds, s, a);
-    if (e != hipSuccess) return e;
-    return launch_args(down, dim3(a.down_tiles, rows, a.sharers), dim3(down_waves * 64), down_waves * down_wave + table, s, a);
+    hipError_t e = hipSuccess;
+    if constexpr (W4) {
+        e = a.gate_up.w4.zeros ? launch_gate_up<T, W4, N2, FOLD, true>(a, s) : launch_gate_up<T, W4, N2, FOLD, false>(a, s);
+        if (e != hipSuccess) return e;
+        return a.down.w4.zeros ? launch_down<T, W4, N2, FOLD, true>(a, s) : launch_down<T, W4, N2, FOLD, false>(a, s);
+    } else {
+        e = launch_gate_up<T, W4, N2, FOLD, false>(a, s);
+        return e != hipSuccess ? e : launch_down<T, W4, N2, FOLD, false>(a, s);
+    }
 }
 
 template <typename T, int N2>
 hipError_t launch_columns(const MoeArgs &a, hipStream_t s)
 {
-    if (!a.group) return launch_experts<T, false, N2, 128, false>(a, s);
-    auto folds = [&](auto n) {
-        return a.gate_up.w4.zeros ? launch_experts<T, true, N2, decltype(n)::value, true>(a, s) : launch_experts<T, true, N2, decltype(n)::value, false>(a, s);
-    };
-    if (a.group % 128 == 0) return folds(std::integral_constant<int, 128>());
-    if (a.group % 64 == 0) return folds(std::integral_constant<int, 64>());
-    return folds(std::integral_constant<int, 32>());
+    if (!a.group) return launch_experts<T, false, N2, 128>(a, s);
+    if (a.group % 128 == 0) return launch_experts<T, true, N2, 128>(a, s);
+    if (a.group % 64 == 0) return launch_experts<T, true, N2, 64>(a, s);
+    return launch_experts<T, true, N2, 32>(a, s);
 }
 
 template <typename T>

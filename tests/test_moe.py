@@ -153,6 +153,17 @@ def test_scores_bias_scalars_zeros_and_rows_inside_larger_arrays(dtype, group, s
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens", [1, 9])
+@pytest.mark.parametrize("zeros", ["gate_up", "down"])
+def test_zero_points_of_one_matrix_alone(dtype, tokens, zeros):
+    p = Problem(dtype, tokens, 96, 64, 6, 2, group=32, zeros=True)
+    other = Problem(dtype, tokens, 96, 64, 6, 2, group=32, seed=1)
+    setattr(p, *(("down", other.down) if zeros == "gate_up" else ("gate_up", other.gate_up)))
+    _check(p)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("group", [0, 32])
 def test_the_largest_counts(group):
     _check(Problem(BF16, G.MOE_MAX_TOKENS, 48, 32, 16, 4, group))
