@@ -40,7 +40,8 @@ __device__ inline float nearest(float w, float s, float by)
     return n;
 }
 
-// Sixteen bytes or the elements of them that exist (here >= 1), as floats in the format's sense; the others are 0.
+// Sixteen bytes or the elements of them that exist, as floats in the format's sense; the others are 0.  (What is finite times 0 is 0, and their sum says so at an
+// instruction an element; one that is not is rare.)
 template <typename TW> constexpr int kPer16 = 16 / (int)sizeof(TW);
 template <typename TW>
 __device__ inline void load_weights(float (&v)[kPer16<TW>], const TW *p, int64_t here)
@@ -55,31 +56,51 @@ __device__ inline void load_weights(float (&v)[kPer16<TW>], const TW *p, int64_t
         for (int i = 0; i < kPer16<TW> - 1; ++i)
             if (i < here) u.e[i] = p[i];
     }
+    float nothing = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPer16<TW>; ++i) v[i] = finite<TW>((float)u.e[i]);
+    for (int i = 0; i < kPer16<TW>; ++i) {
+        v[i] = (float)u.e[i];
+        nothing = __builtin_fmaf(v[i], 0.0f, nothing);
+    }
+    if (nothing != nothing)
+#pragma unroll
+        for (int i = 0; i < kPer16<TW>; ++i) v[i] = finite<TW>(v[i]);
 }
 
-// LANES lanes, neighbours, have a group of a row: each 16 bytes of it a step.  Groups of up to 64 * 16 bytes go by in one step and are read once; longer ones are
-// read twice, the second time from the cache.  Bound by what it reads and writes.
+// LANES lanes, neighbours, have a group of a row: 16 elements each, 16 bytes at a time.  Groups of up to 64 * 16 elements go by in one step and are read once; longer
+// ones are read twice, the second time from the cache.
+// Bound by what it reads and writes, as long as the instructions for an element are few: a division of 64 bits for each 16 bytes' place, a branch for each element's
+// rounding and reductions through LDS made it 69 us for 8192 x 8192 in bf16, groups of 128, of which 168 MB take 33; this is 47 us.
+constexpr int kQuantElements = 16;
 template <typename TW, typename T, int LANES>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
 {
-    constexpr int E = kPer16<TW>;
-    const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LANES, all = (uint64_t)a.m * a.groups;
-    const uint32_t lane = threadIdx.x % LANES;
-    if (at >= all) return;                                          // (the lanes of a group together)
-    const uint64_t i = at / a.groups;
-    const uint32_t g = (uint32_t)(at - i * a.groups);
-    const uint64_t l0 = (uint64_t)g * a.group, l1 = l0 + a.group < a.k ? l0 + a.group : a.k;
-    const TW *w = static_cast<const TW *>(a.W) + i * a.ldw;
-    float low = 0.0f, high = 0.0f, v[E];
-    for (uint64_t l = l0 + lane * E; l < l1; l += LANES * E) {
-        load_weights<TW>(v, w + l, (int64_t)(l1 - l));
+    constexpr int E = kPer16<TW>, PIECES = kQuantElements / E;
+    const uint32_t at = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const uint32_t i = at / a.groups, g = at - i * a.groups;
+    if (i >= a.m) return;                                           // (the lanes of a group together)
+    const uint32_t l0 = g * a.group, length = min(a.group, a.k - l0);
+    const TW *w = static_cast<const TW *>(a.W) + i * a.ldw + l0;
+    float low = 0.0f, high = 0.0f, v[PIECES][E];
+    auto load = [&](uint32_t step) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            low = fminf(low, v[e]);
-            high = fmaxf(high, v[e]);
+        for (int p = 0; p < PIECES; ++p) {
+            const uint32_t l = step + (p * LANES + lane) * E;
+            if (l < length) load_weights<TW>(v[p], w + l, length - l);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[p][e] = 0.0f;
         }
+    };
+    for (uint32_t step = 0; step < length; step += LANES * kQuantElements) {
+        load(step);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                low = fminf(low, v[p][e]);
+                high = fmaxf(high, v[p][e]);
+            }
     }
     for (int d = 1; d < LANES; d <<= 1) {
         low = fminf(low, __shfl_xor(low, d));
@@ -90,31 +111,52 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
     float s = zeros ? (float)(((double)high - (double)low) / 15.0) : fmaxf(high, -low) / 7.0f;
     s = (float)(T)fminf(s, Limits<T>::largest);
     float z = zeros ? 0.0f : kW4Zero;
-    // (scales so small that 1 / s is infinite: as everything by 2^64, which changes no quotient)
-    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, by = 1.0f / su;
+    // (scales so small that 1 / s is infinite: as everything by 2^64, which changes no quotient; without a scale every number is the zero point)
+    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, su = s * up, by = s == 0.0f ? 0.0f : 1.0f / su;
+    const float half = s == 0.0f ? __builtin_inff() : 0.5f * su;
     if (zeros && s != 0.0f) z = fminf(fmaxf(nearest(-low * up, su, by), 0.0f), 15.0f);
     if (lane == 0) {
         static_cast<T *>(const_cast<void *>(a.w.scales))[g + i * a.w.lds] = (T)s;
         if (zeros) const_cast<uint8_t *>(a.w.zeros)[g + i * a.w.ldz] = (uint8_t)z;
     }
-    uint8_t *q = const_cast<uint8_t *>(a.w.q) + i * a.w.ldq;
-    const bool once = l1 - l0 <= LANES * E;
-    for (uint64_t l = l0 + lane * E; l < l1; l += LANES * E) {
-        if (!once) load_weights<TW>(v, w + l, (int64_t)(l1 - l));
-        uint32_t codes = 0;
+    uint8_t *q = const_cast<uint8_t *>(a.w.q) + i * a.w.ldq + l0 / 2;
+    const bool once = length <= LANES * kQuantElements;
+    for (uint32_t step = 0; step < length; step += LANES * kQuantElements) {
+        if (!once) load(step);
+        float n[PIECES][E], worst = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t code = (uint32_t)(s == 0.0f ? z : __builtin_amdgcn_fmed3f(nearest(v[e] * up, su, by) + z, 0.0f, 15.0f));
-            if (l + e < l1) codes |= code << (4 * e);
-        }
-        const uint32_t bytes = (uint32_t)((l1 - l < E ? l1 - l : E) + 1) / 2;
-        typedef uint32_t __attribute__((aligned(1))) u32_any;
-        typedef uint16_t __attribute__((aligned(1))) u16_any;
-        if (bytes == E / 2) {
-            if constexpr (E == 8) *reinterpret_cast<u32_any *>(q + l / 2) = codes;
-            else *reinterpret_cast<u16_any *>(q + l / 2) = (uint16_t)codes;
-        } else {
-            for (uint32_t b = 0; b < bytes; ++b) q[l / 2 + b] = (uint8_t)(codes >> (8 * b));
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[p][e] *= up;
+                n[p][e] = rintf(__builtin_amdgcn_fmed3f(v[p][e] * by, -16.0f, 16.0f));
+                worst = fmaxf(worst, __builtin_fabsf(__builtin_fmaf(-n[p][e], su, v[p][e])));
+            }
+        if (worst >= half)                                          // (one of them on a border, or next to it)
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int e = 0; e < E; ++e) n[p][e] = nearest(v[p][e], su, by);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const uint32_t l = step + (p * LANES + lane) * E;
+            if (l >= length) continue;
+            uint32_t codes = 0;
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {                        // two codes are a byte
+                const float c0 = __builtin_amdgcn_fmed3f(n[p][e] + z, 0.0f, 15.0f), c1 = __builtin_amdgcn_fmed3f(n[p][e + 1] + z, 0.0f, 15.0f);
+                codes = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(c1, 16.0f, c0), e / 2, codes);
+            }
+            const uint32_t here = min(length - l, (uint32_t)E);
+            typedef uint32_t __attribute__((aligned(1))) u32_any;
+            typedef uint16_t __attribute__((aligned(1))) u16_any;
+            if (here == E) {
+                if constexpr (E == 8) *reinterpret_cast<u32_any *>(q + l / 2) = codes;
+                else *reinterpret_cast<u16_any *>(q + l / 2) = (uint16_t)codes;
+            } else {
+                codes &= (1u << (4 * here)) - 1;
+                for (uint32_t b = 0; b < (here + 1) / 2; ++b) q[l / 2 + b] = (uint8_t)(codes >> (8 * b));
+            }
         }
     }
 }
@@ -359,15 +401,16 @@ int mmbo_w4_quantize(int w_dtype, int dtype, size_t m, size_t k, size_t group, c
     const size_t groups = ceil_div(k, group);
     QuantArgs a{matrix_of(Q, ldq, scales, lds, zeros, ldz), const_cast<void *>(W), ldw, 0, (uint32_t)k, (uint32_t)group, (uint32_t)groups};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    // lanes for a group of any size, as many as its 16 bytes: a power of two
-    const size_t wsize = w_dtype == MMBO_F32 ? 4 : 2, pieces = ceil_div(std::min(group, k) * wsize, 16);
-    int lanes = 4;
-    while (lanes < 64 && (size_t)lanes < pieces) lanes *= 2;
+    // lanes for a group of any size: a power of two
+    const size_t wsize = w_dtype == MMBO_F32 ? 4 : 2, most = ceil_div(std::min(group, k), kQuantElements);
+    size_t lanes = 2;
+    while (lanes < 64 && lanes < most) lanes *= 2;
     auto launch = [&](auto *w, auto *t) {
         using TW = std::remove_pointer_t<decltype(w)>;
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid((unsigned)ceil_div(a.m * groups * lanes, 256)), block(256);
-        return lanes == 4    ? launch_args(w4_quantize_kernel<TW, T, 4>, grid, block, 0, s, a)
+        return lanes == 2    ? launch_args(w4_quantize_kernel<TW, T, 2>, grid, block, 0, s, a)
+               : lanes == 4  ? launch_args(w4_quantize_kernel<TW, T, 4>, grid, block, 0, s, a)
                : lanes == 8  ? launch_args(w4_quantize_kernel<TW, T, 8>, grid, block, 0, s, a)
                : lanes == 16 ? launch_args(w4_quantize_kernel<TW, T, 16>, grid, block, 0, s, a)
                : lanes == 32 ? launch_args(w4_quantize_kernel<TW, T, 32>, grid, block, 0, s, a)
