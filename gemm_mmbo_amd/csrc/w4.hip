@@ -40,37 +40,25 @@ __device__ inline float nearest(float w, float s, float by)
     return n;
 }
 
-// Sixteen bytes or the elements of them that exist, as floats in the format's sense; the others are 0.  (What is finite times 0 is 0, and their sum says so at an
-// instruction an element; one that is not is rare.)
+// Sixteen bytes or the elements of them that exist (any number); the others are 0.
 template <typename TW> constexpr int kPer16 = 16 / (int)sizeof(TW);
+typedef u32x4 __attribute__((aligned(1))) u32x4_any;
 template <typename TW>
-__device__ inline void load_weights(float (&v)[kPer16<TW>], const TW *p, int64_t here)
+__device__ inline u32x4 load_part(const TW *p, int64_t here)
 {
-    typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+    if (here >= kPer16<TW>) return *reinterpret_cast<const u32x4_any *>(p);
     union { u32x4 q; TW e[kPer16<TW>]; } u;
-    if (here >= kPer16<TW>) {
-        u.q = *reinterpret_cast<const u32x4_any *>(p);
-    } else {
-        u.q = u32x4{0, 0, 0, 0};
+    u.q = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kPer16<TW> - 1; ++i)
-            if (i < here) u.e[i] = p[i];
-    }
-    float nothing = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer16<TW>; ++i) {
-        v[i] = (float)u.e[i];
-        nothing = __builtin_fmaf(v[i], 0.0f, nothing);
-    }
-    if (nothing != nothing)
-#pragma unroll
-        for (int i = 0; i < kPer16<TW>; ++i) v[i] = finite<TW>(v[i]);
+    for (int i = 0; i < kPer16<TW> - 1; ++i)
+        if (i < here) u.e[i] = p[i];
+    return u.q;
 }
 
 // LANES lanes, neighbours, have a group of a row: 16 elements each, 16 bytes at a time.  Groups of up to 64 * 16 elements go by in one step and are read once; longer
 // ones are read twice, the second time from the cache.
 // Bound by what it reads and writes, as long as the instructions for an element are few: a division of 64 bits for each 16 bytes' place, a branch for each element's
-// rounding and reductions through LDS made it 69 us for 8192 x 8192 in bf16, groups of 128, of which 168 MB take 33; this is 47 us.
+// rounding made it 69 us for 8192 x 8192 in bf16, groups of 128, whose 168 MB take 33; this is 45 us.
 constexpr int kQuantElements = 16;
 template <typename TW, typename T, int LANES>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
@@ -83,14 +71,28 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
     const TW *w = static_cast<const TW *>(a.W) + i * a.ldw + l0;
     float low = 0.0f, high = 0.0f, v[PIECES][E];
     auto load = [&](uint32_t step) {
+        union { u32x4 q; TW e[E]; } u[PIECES];
+        if (step + LANES * kQuantElements <= length) {              // (all pieces under way together)
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const uint32_t l = step + (p * LANES + lane) * E;
-            if (l < length) load_weights<TW>(v[p], w + l, length - l);
-            else
+            for (int p = 0; p < PIECES; ++p) u[p].q = *reinterpret_cast<const u32x4_any *>(w + step + (p * LANES + lane) * E);
+        } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[p][e] = 0.0f;
+            for (int p = 0; p < PIECES; ++p) u[p].q = load_part<TW>(w + step + (p * LANES + lane) * E, (int64_t)length - (step + (p * LANES + lane) * E));
         }
+        // (what is finite times 0 is 0, and their sum says so at an instruction an element; one that is not is rare)
+        float nothing = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[p][e] = (float)u[p].e[e];
+                nothing = __builtin_fmaf(v[p][e], 0.0f, nothing);
+            }
+        if (nothing != nothing)
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[p][e] = finite<TW>(v[p][e]);
     };
     for (uint32_t step = 0; step < length; step += LANES * kQuantElements) {
         load(step);
@@ -176,7 +178,6 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
     const uint8_t *q = a.w.q + i * a.w.ldq + l / 2;
     T *to = static_cast<T *>(a.W) + i * a.ldw + l;
     union { u32x4 v; T e[8]; } u;
-    typedef u32x4 __attribute__((aligned(1))) u32x4_any;
     typedef uint32_t __attribute__((aligned(1))) u32_any;
     if (l + 8 <= a.k) {
         const uint32_t codes = *reinterpret_cast<const u32_any *>(q);
