@@ -224,57 +224,68 @@ __device__ inline void select_token(const MoeArgs &a, uint32_t token, uint32_t l
 // A row's selection in LDS, and what a work-group needs to make its table.
 struct Selection {
     uint16_t *id;                               // of a pair; whole eights of them
+    uint16_t *before;                           // of a part of the pairs, for an expert: pairs by expert in front of it; whole eights
+    uint16_t *jobs_before;                      // of an expert; whole eights
     float *weight;
     uint16_t *pair;                             // pairs by expert
-    uint16_t *before;                           // of a part of the pairs, for an expert: pairs by expert in front of it
-    uint16_t *jobs_before;                      // of an expert
 };
 constexpr uint32_t kMostParts = 512;            // (no work-group has more threads)
+__host__ __device__ inline uint32_t eights(uint32_t n) { return (n + 7) / 8 * 8; }
 __host__ __device__ inline uint32_t select_bytes(uint32_t pairs, uint32_t experts)
 {
-    return ((pairs + 7) / 8 * 16 + pairs * 4 + (pairs + kMostParts + 2 * experts) * 2 + 15) / 16 * 16;
+    return ((eights(pairs) + kMostParts + eights(experts)) * 2 + pairs * 6 + 15) / 16 * 16;
 }
 __device__ inline Selection selection_at(char *lds, uint32_t most_pairs, uint32_t experts)
 {
     Selection s;
     s.id = reinterpret_cast<uint16_t *>(lds);
-    s.weight = reinterpret_cast<float *>(s.id + (most_pairs + 7) / 8 * 8);
+    s.before = s.id + eights(most_pairs);
+    s.jobs_before = s.before + kMostParts;
+    s.weight = reinterpret_cast<float *>(s.jobs_before + eights(experts));
     s.pair = reinterpret_cast<uint16_t *>(s.weight + most_pairs);
-    s.jobs_before = s.pair + most_pairs;
-    s.before = s.jobs_before + experts;
     return s;
 }
 
-// Sums of those in front of each of n numbers (their sum stays below 2^16), by one wavefront; their sum.
+// Sums of those in front of each of n <= 512 numbers (their sum stays below 2^16), by one wavefront, eight to a lane; their sum.  v: whole eights, aligned to them.
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 __device__ inline uint32_t scan(uint16_t *v, uint32_t n, uint32_t lane)
 {
-    uint32_t total = 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-        const uint32_t own = i0 + lane < n ? v[i0 + lane] : 0;
-        uint32_t sum = own;
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t other = __shfl_up(sum, d);
-            if ((int)lane >= d) sum += other;
+    u16x8 *const mine = reinterpret_cast<u16x8 *>(v) + lane;
+    uint32_t own[8] = {}, sum = 0;
+    if (lane * 8 < n) {
+        const u16x8 q = *mine;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            own[i] = sum;
+            if (lane * 8 + i < n) sum += q[i];
         }
-        if (i0 + lane < n) v[i0 + lane] = (uint16_t)(total + sum - own);
-        total += __builtin_amdgcn_readlane(sum, 63);
     }
-    return total;
+    uint32_t all = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t other = __shfl_up(all, d);
+        if ((int)lane >= d) all += other;
+    }
+    if (lane * 8 < n) {
+        u16x8 q;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = (uint16_t)(all - sum + own[i]);
+        *mine = q;
+    }
+    return __builtin_amdgcn_readlane(all, 63);
 }
 
 // The table of `pairs` pairs, by a work-group that has them in LDS.  A thread looks through a part of the pairs for an expert's, eight ids at a time: one thread
 // to an expert, and a store to memory a pair, was 12 us for 128 pairs.
 __device__ inline void make_table(const MoeArgs &a, uint32_t pairs, const Selection &sel, const Table &table)
 {
-    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     const u16x8 *const id8 = reinterpret_cast<const u16x8 *>(sel.id);
-    const uint32_t eights = (pairs + 7) / 8, parts = max(min(blockDim.x / a.experts, eights), 1u);
-    if (threadIdx.x < eights * 8 - pairs) sel.id[pairs + threadIdx.x] = 0xFFFF;
+    const uint32_t pieces = (pairs + 7) / 8, parts = max(min(blockDim.x / a.experts, pieces), 1u);
+    if (threadIdx.x < pieces * 8 - pairs) sel.id[pairs + threadIdx.x] = 0xFFFF;
     __syncthreads();
     for (uint32_t x = threadIdx.x; x < a.experts * parts; x += blockDim.x) {
         const uint32_t e = x / parts, part = x % parts;
         uint32_t n = 0;
-        for (uint32_t q = eights * part / parts; q < eights * (part + 1) / parts; ++q) {
+        for (uint32_t q = pieces * part / parts; q < pieces * (part + 1) / parts; ++q) {
             const u16x8 v = id8[q];
 #pragma unroll
             for (int i = 0; i < 8; ++i) n += v[i] == e;
@@ -290,7 +301,7 @@ __device__ inline void make_table(const MoeArgs &a, uint32_t pairs, const Select
         if (part == 0) sel.jobs_before[e] = (uint16_t)((end_of(e) - sel.before[x] + a.columns - 1) / a.columns);
         uint32_t at = sel.before[x];
         if (at == (x + 1 < a.experts * parts ? (uint32_t)sel.before[x + 1] : pairs)) continue;
-        for (uint32_t q = eights * part / parts; q < eights * (part + 1) / parts; ++q) {
+        for (uint32_t q = pieces * part / parts; q < pieces * (part + 1) / parts; ++q) {
             const u16x8 v = id8[q];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -371,7 +382,9 @@ __device__ inline Table stage_table(const MoeArgs &a, uint32_t row, char *lds)
     return table_at(lds, most_pairs, a.most_jobs);
 }
 
-constexpr uint32_t kSelfSelect = 4;             // tokens that are selected by the work-groups of the first product: a launch less
+// Tokens that every work-group of the first product selects for itself, a wavefront each: a launch less (8 tokens, 8 of 64 experts of 2048 x 1024 in 4 bits: 59.9 us, with
+// a launch for it 61.4).
+constexpr uint32_t kSelfSelect = 8;
 constexpr int kMoeWaves = 8;                    // or as many as fit the LDS
 constexpr unsigned kLds = 160 * 1024;
 
