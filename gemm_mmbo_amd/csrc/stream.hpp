@@ -14,6 +14,10 @@
 // One MFMA against ones sums the columns' elements of a group; zero point (+ 128) times that comes off the group's sums, which then are multiplied by
 // its scale, in fp32.  The sums lose five bits of fp32's 24 to the 128 at most, of which a store to bf16 keeps 8.
 // 16-bit weights: a block is 64 places, a line of a row.
+//
+// What bounds it: one column, the weights from memory beside requests of scales, a line a row and block (28672 x 1 x 8192: fp16 31 us, bf16 with zero points 35, 121 MB
+// take 21; 4096 x 1 x 4096 4.9 us, a launch).  More columns, what a CU gets from the L2, some 50 bytes a ns: each work-group reads all columns for its 16 or 32 rows
+// (4096 x 16 x 14336 12.9 us for 0.6 MB a CU, 8192 x 64 x 8192 27.1 for 1.3 MB).
 #pragma once
 
 #include <type_traits>

@@ -2,7 +2,6 @@
 #include "../../include/mmbo_gemm.h"
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "w4_tile.hpp"
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
     }
 }
 
-// A thread: 32 places of a row, with one scale.
+// Four threads have 32 places of a row, with one scale.  Bound by what it reads and writes: 8192 x 8192 in groups of 128, 168 MB, 30 us (5.6 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
 {
@@ -188,8 +187,6 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
         for (uint32_t e = 0; l + e < a.k; ++e) to[e] = (T)(((float)(e & 1 ? q[e / 2] >> 4 : q[e / 2] & 15) - z) * s);
     }
 }
-
-constexpr size_t kMaxDim = 0x7FFFFFFFull;
 
 // What the three calls check of a weight's sizes.
 int check_weight(size_t m, size_t k, size_t group, size_t ldq, size_t lds, const void *zeros, size_t ldz)
@@ -219,19 +216,7 @@ int by_rows(size_t m, size_t threads, const Launch &launch)
     return MMBO_OK;
 }
 
-template <typename Kernel>
-hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
-{
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess || (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire))) return e;
-    e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e == hipSuccess && dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
-    return e;
-}
-
 constexpr int kStreamWaves = 8;
-
 
 template <typename T, int N2, int FT, int FOLD, bool ZEROS>
 hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
@@ -240,13 +225,13 @@ hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
     // with rings of 3, 33.7 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 with rings of 2, 13.6 of 3, 14.5 of 4.
     constexpr int DEPTH = N2 == 1 ? 3 : 2;
     typedef stream::Stream<T, true, N2, FT, 1, FOLD, ZEROS, DEPTH> S;
-    constexpr int kWaveBytes = S::LDS_BYTES + 2 * S::SET_FLOATS * 4, kMost = std::min(kStreamWaves, 160 * 1024 / kWaveBytes);
+    constexpr int kWaveBytes = S::LDS_BYTES + 2 * S::SET_FLOATS * 4, kMost = std::min<int>(kStreamWaves, kLds / kWaveBytes);
     static std::atomic<bool> set[64];
     auto kernel = gemm_w4_stream_kernel<T, N2, FT, FOLD, ZEROS, DEPTH>;
     if (hipError_t e = allow_lds(kernel, set)) return e;
     const int waves = (int)std::max<uint32_t>(std::min<uint32_t>(S::blocks_of(a.k), kMost), 1);
     // as many work-groups as the CUs hold at a time, two of eight wavefronts each at most (128256 x 1 x 4096: one 68, two 58, three 58 us)
-    const unsigned columns = (unsigned)ceil_div(a.n, N2), held = 256 * std::min<unsigned>(160 * 1024 / (waves * kWaveBytes), 2 * kStreamWaves / waves);
+    const unsigned columns = (unsigned)ceil_div(a.n, N2), held = 256 * std::min<unsigned>(kLds / (waves * kWaveBytes), 2 * kStreamWaves / waves);
     const unsigned groups = (unsigned)std::min<size_t>(ceil_div(a.m, 16 * FT), std::max(held / columns, 1u));
     return launch_args(kernel, dim3(groups, columns), dim3(waves * 64), waves * kWaveBytes, s, a);
 }
@@ -280,10 +265,10 @@ hipError_t launch_tile_kernel(const GemmW4Args &a, hipStream_t s)
     if constexpr (!C::FITS) {                    // (eight wavefronts with four scales and zero points a slot)
         return launch_tile_kernel<T, WM / 2, NC, FOLDS, ZEROS>(a, s);
     } else {
-    static std::atomic<bool> set[64];
-    auto kernel = gemm_w4_tile_kernel<T, WM, NC, FOLDS, ZEROS, 3>;
-    if (hipError_t e = allow_lds(kernel, set)) return e;
-    return launch_args(kernel, dim3((unsigned)(ceil_div(a.m, C::ROWS) * ceil_div(a.n, C::COLUMNS))), dim3(C::THREADS), C::LDS_BYTES, s, a);
+        static std::atomic<bool> set[64];
+        auto kernel = gemm_w4_tile_kernel<T, WM, NC, FOLDS, ZEROS, 3>;
+        if (hipError_t e = allow_lds(kernel, set)) return e;
+        return launch_args(kernel, dim3((unsigned)(ceil_div(a.m, C::ROWS) * ceil_div(a.n, C::COLUMNS))), dim3(C::THREADS), C::LDS_BYTES, s, a);
     }
 }
 
@@ -301,7 +286,7 @@ hipError_t launch_tile(const GemmW4Args &a, hipStream_t s)
 // More than 32 columns: what a call takes by each kernel, in us, from rounds of work-groups over the 256 CUs.  Measured, fp16 and bf16, group 128:
 //   stream, 32 x 32 (or 16 x 32): what a work-group pulls at some 47 bytes a ns    128 x 4096 x 4096 17.3, 256 30-32, 512 57-61; 64 x 8192 x 8192 29
 //   tile of 64 x 64, two a CU: 1.1 us a slot of 128 places, 1.4 for a CU with two   256 x 8192 x 4096 45, 512 x 4096 x 4096 45, 1024 87
-//   tile of 256 x 128: 2.1 us a slot                                               512 x 4096 x 4096 64, 1024 66, 2048 x 8192 x 4096 136 and 146
+//   tile of 256 x 128: 2.1 us a slot                                               512 x 4096 x 4096 64, 1024 66, 2048 x 8192 x 4096 137 and 147
 enum class Kernel { kStream16, kStream32, kTile64, kTile256 };
 Kernel kernel_for(size_t m, size_t n, size_t k)
 {

@@ -2,6 +2,8 @@
 // (l, i): place l of k of row i.  Code (l, i) is half of byte (l + i * ldq) / 2, the low half for even l.
 #pragma once
 
+#include <atomic>
+
 #include "launch.hpp"
 
 namespace mmbo {
@@ -38,6 +40,9 @@ struct QuantArgs {
     uint32_t m, k, group, groups;
 };
 
+constexpr size_t kMaxDim = 0x7FFFFFFFull;
+constexpr unsigned kLds = 160 * 1024;           // of a CU
+
 template <typename N>
 constexpr size_t ceil_div(size_t n, N by) { return (n + by - 1) / by; }
 
@@ -48,6 +53,18 @@ inline hipError_t launch_args(Kernel kernel, dim3 grid, dim3 block, unsigned lds
 {
     void *kargs[] = {const_cast<Args *>(&args)};
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, kargs, lds_bytes, stream);
+}
+
+// All of a CU's LDS to a kernel, asked for once a device.
+template <typename Kernel>
+hipError_t allow_lds(Kernel kernel, std::atomic<bool> (&set)[64])
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire))) return e;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e == hipSuccess && dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+    return e;
 }
 
 }  // namespace mmbo
