@@ -172,6 +172,47 @@ def test_the_largest_counts(group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [0, 64])
+@pytest.mark.parametrize("tokens,experts,top_k", [(5, 16, 2), (8, G.MOE_MAX_EXPERTS, G.MOE_MAX_TOP_K), (9, G.MOE_MAX_EXPERTS, G.MOE_MAX_TOP_K), (8, 1, 1), (8, 4, 1),
+                                                  (7, 65, 3), (64, 128, 2), (65, 128, 4), (64, 128, 5)])
+def test_where_the_selection_and_the_jobs_change_their_form(group, tokens, experts, top_k):
+    """Up to 8 tokens and more; jobs of four columns (up to two pairs to an expert) and of sixteen."""
+    _check(Problem(BF16, tokens, 72, 40, experts, top_k, group))
+    _check(Problem(F16, tokens, 136, 24, experts, top_k, group, zeros=True, sigmoid=True, beta=0.5, pad=8))
+
+
+@pytest.mark.gpu
+def test_one_workspace_for_calls_one_behind_the_other():
+    """Layers of different sizes and numbers of tokens over the same memory, as a program's layers share it: eager, and captured into one graph."""
+    problems = [Problem(F16, t, h, i, e, k, group) for t, h, i, e, k, group in
+                ((40, 96, 64, 8, 2, 0), (1, 160, 48, 32, 4, 32), (8, 64, 32, 64, 8, 0), (9, 64, 32, 64, 8, 64), (70, 80, 24, 5, 3, 0))]
+    layers = [p.layer() for p in problems]
+    nbytes = max(G.moe_workspace_bytes(layer, p.tokens) for layer, p in zip(layers, problems))
+    ws = torch.full((nbytes,), 0xEE, dtype=torch.uint8, device="cuda")
+    xs, ys = [p.x.cuda() for p in problems], [torch.empty((p.tokens, p.hidden), dtype=torch.float16, device="cuda") for p in problems]
+
+    def calls(stream):
+        for p, layer, x, y in zip(problems, layers, xs, ys):
+            G.moe(layer, p.tokens, 1.0, x, p.hidden, 0.0, y, p.hidden, ws, nbytes, stream=stream)
+
+    alone = [p.run()[0] for p in problems]
+    for _ in range(2):
+        calls(None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(y.cpu(), a) for y, a in zip(ys, alone))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(torch.cuda.current_stream())
+    for _ in range(3):
+        for y in ys:
+            y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y.cpu(), a) for y, a in zip(ys, alone))
+        ws.fill_(0xFF)
+
+
+@pytest.mark.gpu
 def test_ties_go_to_the_lower_expert():
     p = Problem(F16, 9, 64, 32, 96, 6)
     p.router[:] = p.router[0]                       # every expert the same logit
