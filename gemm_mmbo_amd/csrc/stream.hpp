@@ -158,7 +158,8 @@ struct Stream {
                          X_LOADS = (X_LINES * N2 * 8 + 63) / 64, X_PLANE = X_LINES * N2 * 128;
     static constexpr int S_LOADS = W4 ? (FOLDS + 3) / 4 : 0, S_TILE = FOLDS * 64;
     static constexpr int X_AT = FT * W_TILE, S_AT = X_AT + PLANES * X_PLANE, Z_AT = S_AT + (W4 ? FT * S_TILE : 0), SLOT = (Z_AT + (W4 && ZEROS ? FT * S_TILE : 0) + 127) / 128 * 128;
-    static constexpr int LOADS = FT * WP + PLANES * X_LOADS + FT * S_LOADS * (ZEROS ? 2 : 1);
+    static constexpr bool S_ONE = W4 && FT * FOLDS <= 4;          // one load has the scales of all tiles (8192 x 16 x 8192 11.5 us, with one a tile 12.2)
+    static constexpr int LOADS = FT * WP + PLANES * X_LOADS + (S_ONE ? 1 : FT * S_LOADS) * (ZEROS ? 2 : 1);
     static constexpr int LDS_BYTES = (DEPTH * SLOT + 1023) / 1024 * 1024;
     static_assert((DEPTH - 1) * LOADS < 64, "vmcnt counts to 63");
     typedef f32x4 Sums[NT][FT];
@@ -240,9 +241,14 @@ struct Stream {
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) from.x[q][p] += b * BLOCK + x_chunk(lane, p) * 8 + (N2 < 8 ? x_line(lane, 0) : 0);
         }
+        if constexpr (S_ONE && FT == 2)
+            if (lane >= 16 * FOLDS) {
+                from.scales[0] = from.scales[1];
+                if constexpr (ZEROS) from.zeros[0] = from.zeros[1];
+            }
 #pragma unroll
         for (int j = 0; j < S_LOADS; ++j) {
-            const uint32_t at = b * STEPS + (j * 4 + (lane >> 4)) * (STEPS / FOLDS);
+            const uint32_t at = b * STEPS + (S_ONE ? (lane >> 4) % FOLDS : j * 4 + (lane >> 4)) * (STEPS / FOLDS);
             group[j] = at / group32;
             rest[j] = at % group32;
         }
@@ -256,13 +262,13 @@ struct Stream {
             enter_job(enter);
         }
         const uint32_t to = lds_at + slot * SLOT;
-        // scales: lane's row lane % 16, its folds lane / 16 and every fourth behind that
+        // scales: lane's row lane % 16, its folds lane / 16 and every fourth behind that; or in one load tile lane / (16 * FOLDS), fold lane / 16 % FOLDS
 #pragma unroll
         for (int j = 0; j < S_LOADS; ++j) {
             const uint32_t g = min(group[j], (k - 1) / 32 / group32);
-            if (FOLDS >= 4 || lane < 16 * FOLDS)
+            if (lane < 16 * FOLDS * (S_ONE ? FT : 1) || FOLDS >= 4)
 #pragma unroll
-                for (int f = 0; f < FT; ++f) {
+                for (int f = 0; f < (S_ONE ? 1 : FT); ++f) {
                     direct_load_u16(from.scales[f] + g, to + S_AT + f * S_TILE + j * 256);
                     if constexpr (ZEROS) direct_load_u8(from.zeros[f] + g, to + Z_AT + f * S_TILE + j * 256);
                 }
