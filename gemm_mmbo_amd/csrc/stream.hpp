@@ -9,10 +9,11 @@
 // (4096 x 16 x 14336 in 4 bits: 24 us), with 64 bytes to four lanes 20 (13.3 us), though halves of a line were asked for one behind the other.
 //
 // 4-bit weights: a block is 128 places, half a line of a row (whole lines took longer: 28672 x 1 x 8192 33 us, with half of them 28).  Eight codes become numbers by moving nibbles to where a mantissa ends:
-//   fp16: the code itself, as a subnormal number (code * 2^-24; MFMAs take those as they are): 7 instructions.
-//   bf16: 128 + code, the largest such number with 4 free bits: 9 instructions.
-// One MFMA against ones sums the columns' elements of a group; zero point (+ 128) times that comes off the group's sums, which then are multiplied by
-// its scale, in fp32.  The sums lose five bits of fp32's 24 to the 128 at most, of which a store to bf16 keeps 8.
+//   fp16: a subnormal number, code * 2^-24, of which a packed fma makes (code - zero) * 2^-10: 11 instructions.  Not the subnormal numbers themselves: an MFMA lines its
+//     products up by the operands' exponents, which are then 10 to 13 above the products, and cuts off what fp32 would hold (one in twenty of a product's results was another fp16 number).
+//   bf16: 128 + code, the largest such number with 4 free bits: 9 instructions.  One MFMA against ones sums the columns' elements of a group; (zero point + 128) times that
+//     comes off the group's sums.
+// A group's sums are multiplied by its scale, in fp32.
 // 16-bit weights: a block is 64 places, a line of a row.
 //
 // What bounds it: one column, the weights from memory beside requests of scales, a line a row and block (28672 x 1 x 8192: fp16 31 us, bf16 with zero points 35, 121 MB
@@ -31,6 +32,7 @@ namespace stream {
 
 typedef u32x4 __attribute__((aligned(1))) u32x4_any;
 typedef uint32_t __attribute__((aligned(1))) u32_any;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <typename T> struct Type;
 template <> struct Type<half_t> {
@@ -71,33 +73,41 @@ __device__ inline u32x4 load32_codes(const uint8_t *p, int64_t here)
     return u.v;
 }
 
-// Eight numbers from a dword of codes.  Number n stands for (code + kBias) * kUnit.
+// Eight numbers from a dword of codes.  Number n stands for (n / kUnit - kBias) + kLessZero * zero.
 template <typename T> struct Codes;
 template <> struct Codes<half_t> {
-    static constexpr float kBias = 0.0f, kUnit = 0x1p-24f;
-    struct Masks {};
-    __device__ static inline Masks masks() { return Masks{}; }
-    __device__ static inline f16x8 expand(uint32_t x, const Masks &)
+    static constexpr bool kLessZero = true;
+    static constexpr float kBias = 0.0f, kUnit = 0x1p-10f;
+    typedef f16x2 Zero;
+    __device__ static inline Zero zero_of(uint32_t z)
     {
-        union { uint32_t d[4]; f16x8 v; } u;
+        const half_t v = (half_t)((float)z * -kUnit);
+        return Zero{v, v};
+    }
+    __device__ static inline f16x8 expand(uint32_t x, const Zero &z)
+    {
+        union { f16x2 h[4]; f16x8 v; } u;
         const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
+        const f16x2 up = {(half_t)0x1p14f, (half_t)0x1p14f};
 #pragma unroll
-        for (int p = 0; p < 4; ++p) u.d[p] = __builtin_amdgcn_perm(odd, even, 0x0c040c00u + p * 0x00010001u);       // byte p of either
+        for (int p = 0; p < 4; ++p)                     // byte p of either
+            u.h[p] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(odd, even, 0x0c040c00u + p * 0x00010001u)), up, z);
         return u.v;
     }
 };
 template <> struct Codes<bf16_t> {
+    static constexpr bool kLessZero = false;
     static constexpr float kBias = 128.0f, kUnit = 1.0f;
     // (in registers: with both constants in the instruction it would be two)
-    struct Masks { uint32_t keep, exponent; };
-    __device__ static inline Masks masks()
+    struct Zero { uint32_t keep, exponent; };
+    __device__ static inline Zero zero_of(uint32_t)
     {
-        Masks m{0x000F000Fu, 0x43004300u};
+        Zero m{0x000F000Fu, 0x43004300u};
         asm("" : "+s"(m.keep));
         asm("" : "+v"(m.exponent));
         return m;
     }
-    __device__ static inline bf16x8 expand(uint32_t x, const Masks &m)
+    __device__ static inline bf16x8 expand(uint32_t x, const Zero &m)
     {
         union { uint32_t d[4]; bf16x8 v; } u;
         const uint32_t odd = x >> 4;
@@ -150,7 +160,7 @@ template <typename T, bool W4, int N2, int FT, int PLANES, int FOLD, bool ZEROS,
 struct Stream {
     static_assert(N2 == 1 || N2 == 4 || N2 == 16 || N2 == 32, "");
     typedef typename Type<T>::Frag Frag;
-    typedef typename Codes<T>::Masks Masks;
+    typedef typename Codes<T>::Zero Zero;
     static constexpr int NT = N2 > 16 ? N2 / 16 : 1, BLOCK = W4 ? 128 : 64, STEPS = BLOCK / 32, ROW_BYTES = W4 ? BLOCK / 2 : 128;
     static constexpr int FOLDS = W4 ? BLOCK / FOLD : 1;
     static constexpr int WP = ROW_BYTES / 64, W_TILE = WP * 1024;
@@ -211,7 +221,6 @@ struct Stream {
     Job from;
     uint32_t r_job, r_block, group[S_LOADS + 1], rest[S_LOADS + 1];                     // (of the lane's folds)
     // products
-    Masks masks;
     struct Operands {
         Frag x[PLANES][STEPS][NT];
         u32x4 w[W4 ? 1 : STEPS][FT];
@@ -221,7 +230,7 @@ struct Stream {
 
     __device__ inline Stream(uint32_t k, uint32_t group32, uint32_t block0, uint32_t per_job, char *lds, int lane)
         : k(k), group32(group32), lds(lds), lane(lane), lds_at(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)MMBO_LDS_PTR(lds))), block0(block0),
-          per_job(per_job), masks(Codes<T>::masks())
+          per_job(per_job)
     {
     }
 
@@ -358,18 +367,26 @@ struct Stream {
             for (int q = 0; q < FOLDS; ++q) {
                 Sums part;
                 f32x4 sums[NT];                  // of the columns' elements
+                uint32_t z[FT];
+                Zero zero[FT];
                 clear(part);
 #pragma unroll
                 for (int c = 0; c < NT; ++c) sums[c] = f32x4{0, 0, 0, 0};
 #pragma unroll
+                for (int f = 0; f < FT; ++f) {
+                    z[f] = ZEROS ? o.zeros[q][f] & kW4ZeroMask : (uint32_t)kW4Zero;
+                    zero[f] = Codes<T>::zero_of(z[f]);
+                }
+#pragma unroll
                 for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i) {
+                    if constexpr (!Codes<T>::kLessZero)
 #pragma unroll
-                    for (int c = 0; c < NT; ++c)
+                        for (int c = 0; c < NT; ++c)
 #pragma unroll
-                        for (int e = 0; e < PLANES; ++e) sums[c] = Type<T>::mfma(o.x[e][i][c], ones<T>(), sums[c]);
+                            for (int e = 0; e < PLANES; ++e) sums[c] = Type<T>::mfma(o.x[e][i][c], ones<T>(), sums[c]);
 #pragma unroll
                     for (int f = 0; f < FT; ++f) {
-                        const Frag w = Codes<T>::expand(o.codes[i][f], masks);
+                        const Frag w = Codes<T>::expand(o.codes[i][f], zero[f]);
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -380,11 +397,12 @@ struct Stream {
                 for (int f = 0; f < FT; ++f) {
                     // the scale of a number, and the number that stands for 0
                     const float s = (float)__builtin_bit_cast(T, (uint16_t)o.scales[q][f]) * (1.0f / Codes<T>::kUnit);
-                    const float z = ((ZEROS ? (float)(o.zeros[q][f] & kW4ZeroMask) : kW4Zero) + Codes<T>::kBias) * Codes<T>::kUnit;
+                    const float n0 = Codes<T>::kLessZero ? 0.0f : (float)z[f] + Codes<T>::kBias;
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[c][f][r] = __builtin_fmaf(s, __builtin_fmaf(-z, sums[c][r], part[c][f][r]), acc[c][f][r]);
+                        for (int r = 0; r < 4; ++r)
+                            acc[c][f][r] = __builtin_fmaf(s, Codes<T>::kLessZero ? part[c][f][r] : __builtin_fmaf(-n0, sums[c][r], part[c][f][r]), acc[c][f][r]);
                 }
             }
         } else {

@@ -3,8 +3,8 @@
 // A wavefront expands its own rows' codes -- no row's is expanded twice in a work-group -- and multiplies them with all of the tile's columns, on the
 // MFMAs and in the layout of stream.hpp.  Codes, scales and columns go through a ring of DEPTH slots of 128 places in LDS that direct loads fill, one barrier
 // a slot.  A code becomes the exact number code - zero:
-//   fp16: a subnormal number (code * 2^-24), from which a packed addition takes zero * 2^-24: 11 instructions for eight.
-//   bf16: from that subnormal number one mixed-precision fma makes code - zero in fp32, and two of those are packed: 19.
+//   fp16: times 2^-10, as in stream.hpp: 11 instructions for eight.
+//   bf16: from the subnormal fp16 number code * 2^-24 one mixed-precision fma makes code - zero in fp32, and two of those are packed: 19.
 // A group's sums, in fp32, are multiplied by its scale and added to the total.  What bounds it is the issue of vector instructions beside the MFMAs: 16
 // MFMAs of 16 clocks a step of 32 places, and for those two wavefronts of a SIMD 2 * (38 (fp16: 22) + 16 + 16) issues of 4.
 // 8192 x 2048 x 4096 in groups of 128: fp16 137 us, bf16 147, 1.0 and 0.94 PFLOP/s; groups of 64 151 and 163, of 32 166 (fp16).
@@ -21,28 +21,13 @@ using namespace stream;
 constexpr int BLOCK = 128, STEPS = 4;
 
 template <typename T> struct Exact;
-template <> struct Exact<half_t> {
-    static constexpr float kUnit = 0x1p-24f;
-    typedef uint32_t Zero;
-    __device__ static inline Zero zero_of(uint32_t z) { return z | z << 16; }       // z * 2^-24, twice
-    __device__ static inline f16x8 expand(uint32_t x, Zero z)
-    {
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        union { f16x2 h[4]; f16x8 v; } u;
-        const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-            u.h[p] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(odd, even, 0x0c040c00u + p * 0x00010001u)) - __builtin_bit_cast(f16x2, z);
-        return u.v;
-    }
-};
+template <> struct Exact<half_t> : Codes<half_t> {};
 template <> struct Exact<bf16_t> {
     static constexpr float kUnit = 1.0f;
     typedef float Zero;
     __device__ static inline Zero zero_of(uint32_t z) { return -(float)z; }
     __device__ static inline bf16x8 expand(uint32_t x, Zero z)
     {
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
         bf16x8 v;
         const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
 #pragma unroll

@@ -1,0 +1,72 @@
+"""Products with 4-bit weights whose every term, (code - zero) * element, and whose sums of any of them are whole numbers below 2^23, a bit less than fp32 holds: whatever
+the order, the sum in fp32 is exact, and the result is that sum times a power of two, with beta C, rounded once.  It has to be equal: what a kernel makes of the codes may not
+cost the sums any of fp32's bits.  In numbers that stand for more than code - zero -- the code and 128, say, whose columns' sums then come off -- the sums pass 2^24."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import gemm_mmbo_amd as G
+import w4_reference as R
+from gemm_mmbo_amd import api
+
+F16, BF16 = G.F16, G.BF16
+UNIT = {F16: 2.0 ** -8, BF16: 1.0}                  # alpha or the scales: fp16 ends at 65504
+
+
+def _problem(dtype, m, n, k, group, zeros):
+    """Weights of scale 1, columns whose runs of 128 have one sign and a large element among small odd ones, and the exact products."""
+    g = torch.Generator().manual_seed(m + n + k + group)
+    w = R.Weight(g, dtype, m, k, group, zeros)
+    w.scales[:] = 1.0
+    b = torch.randint(0, 8, (n, k), generator=g) * 2 + 1
+    b[:, ::4] = torch.randint(128, 256, b[:, ::4].shape, generator=g) * 64              # 8 bits: exact in bf16
+    b[:, (torch.arange(k) // 128) % 2 == 1] *= -1
+    value = w.parts()[0]
+    assert (np.abs(b.numpy()) @ np.abs(value).T).max() < 2 ** 23
+    return w, b.to(R.TORCH[dtype]), b.double().numpy() @ value.T
+
+
+def _rounded(v, dtype):
+    assert np.array_equal(torch.from_numpy(v).float().double().numpy(), v)              # (exact in fp32: the type's rounding is the only one)
+    return torch.from_numpy(v).to(R.TORCH[dtype]).double().numpy()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 16, 32, 40, 150])
+@pytest.mark.parametrize("dtype", [F16])
+def test_sums_that_fp32_holds_are_exact(dtype, n, zeros, group):
+    """C takes off what the type has of the result, and the lowest bits remain."""
+    for m, k in ((200, 256), (33, 201), (130, 64)):
+        w, b, exact = _problem(dtype, m, n, k, group, zeros)
+        c = torch.from_numpy(-UNIT[dtype] * exact).to(R.TORCH[dtype])
+        want = _rounded(UNIT[dtype] * exact + c.double().numpy(), dtype)
+        q, s, z, db, dc = w.q.cuda(), w.scales.cuda(), None if w.zeros is None else w.zeros.cuda(), b.cuda(), c.cuda()
+        torch.cuda.synchronize()
+        G.gemm_w4(dtype, m, n, k, group, UNIT[dtype], q, w.ldq, s, w.lds, z, w.lds, db, k, 1.0, dc, m)
+        torch.cuda.synchronize()
+        off = dc.cpu().double().numpy() - want
+        assert not off.any(), f"{m} x {n} x {k}: {np.mean(off != 0):.2g} of all, by up to {np.abs(off).max() / UNIT[dtype]} of {np.abs(exact).max()}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel,dtype", [(0, F16), (1, F16), (2, F16), (3, F16), (2, BF16), (3, BF16)])
+def test_sums_that_fp32_holds_are_exact_in_every_kernel(kernel, dtype):
+    """Each of the kernels that a call with more than 32 columns may be given."""
+    f = api.lib().mmbo_internal_gemm_w4
+    f.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_size_t] * 4 + [ctypes.c_void_p] * 6
+    for group, zeros in ((32, True), (64, False), (128, True)):
+        m, n, k = 170, 140, 250
+        w, b, exact = _problem(dtype, m, n, k, group, zeros)
+        w.scales[:] = UNIT[dtype]
+        want = _rounded(UNIT[dtype] * exact, dtype)
+        q, s, z, db = w.q.cuda(), w.scales.cuda(), w.zeros.cuda() if zeros else None, b.cuda()
+        dc = torch.full((n, m), float("nan"), dtype=R.TORCH[dtype], device="cuda")
+        torch.cuda.synchronize()
+        assert f(kernel, dtype, m, n, k, group, q.data_ptr(), s.data_ptr(), z.data_ptr() if zeros else None, db.data_ptr(), dc.data_ptr(), None) == 0
+        torch.cuda.synchronize()
+        off = dc.cpu().double().numpy() - want
+        assert not off.any(), f"groups of {group}: {np.mean(off != 0):.2g} of all, by up to {np.abs(off).max() / UNIT[dtype]}"
