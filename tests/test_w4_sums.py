@@ -15,17 +15,23 @@ F16, BF16 = G.F16, G.BF16
 UNIT = {F16: 2.0 ** -8, BF16: 1.0}                  # alpha or the scales: fp16 ends at 65504
 
 
-def _problem(dtype, m, n, k, group, zeros):
-    """Weights of scale 1, columns whose runs of 128 have one sign and a large element among small odd ones, and the exact products."""
+ELEMENTS = {"many": (4, 64, 1.0), "few": (32, 256, 2.0 ** -14)}      # every how many-th is large, 128 to 255 of what, the others' unit (fp16: the smallest normal number)
+
+
+def _problem(dtype, m, n, k, group, zeros, elements="many"):
+    """Weights of scale 1, columns whose runs of 128 have one sign and large elements among small odd ones, and the exact products, in units."""
     g = torch.Generator().manual_seed(m + n + k + group)
     w = R.Weight(g, dtype, m, k, group, zeros)
     w.scales[:] = 1.0
+    every, step, unit = ELEMENTS[elements]
     b = torch.randint(0, 8, (n, k), generator=g) * 2 + 1
-    b[:, ::4] = torch.randint(128, 256, b[:, ::4].shape, generator=g) * 64              # 8 bits: exact in bf16
+    b[:, ::every] = torch.randint(128, 256, b[:, ::every].shape, generator=g) * step    # 8 bits: exact in bf16
     b[:, (torch.arange(k) // 128) % 2 == 1] *= -1
     value = w.parts()[0]
     assert (np.abs(b.numpy()) @ np.abs(value).T).max() < 2 ** 23
-    return w, b.to(R.TORCH[dtype]), b.double().numpy() @ value.T
+    held = (b * unit).to(R.TORCH[dtype])
+    assert torch.equal(held.double(), b.double() * unit)
+    return w, held, b.double().numpy() @ value.T
 
 
 def _rounded(v, dtype):
@@ -38,15 +44,16 @@ def _rounded(v, dtype):
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("n", [1, 3, 16, 32, 40, 150])
 @pytest.mark.parametrize("dtype", [F16])
-def test_sums_that_fp32_holds_are_exact(dtype, n, zeros, group):
+@pytest.mark.parametrize("elements", ["many", "few"])
+def test_sums_that_fp32_holds_are_exact(elements, dtype, n, zeros, group):
     """C takes off what the type has of the result, and the lowest bits remain."""
     for m, k in ((200, 256), (33, 201), (130, 64)):
-        w, b, exact = _problem(dtype, m, n, k, group, zeros)
+        w, b, exact = _problem(dtype, m, n, k, group, zeros, elements)
         c = torch.from_numpy(-UNIT[dtype] * exact).to(R.TORCH[dtype])
         want = _rounded(UNIT[dtype] * exact + c.double().numpy(), dtype)
         q, s, z, db, dc = w.q.cuda(), w.scales.cuda(), None if w.zeros is None else w.zeros.cuda(), b.cuda(), c.cuda()
         torch.cuda.synchronize()
-        G.gemm_w4(dtype, m, n, k, group, UNIT[dtype], q, w.ldq, s, w.lds, z, w.lds, db, k, 1.0, dc, m)
+        G.gemm_w4(dtype, m, n, k, group, UNIT[dtype] / ELEMENTS[elements][2], q, w.ldq, s, w.lds, z, w.lds, db, k, 1.0, dc, m)
         torch.cuda.synchronize()
         off = dc.cpu().double().numpy() - want
         assert not off.any(), f"{m} x {n} x {k}: {np.mean(off != 0):.2g} of all, by up to {np.abs(off).max() / UNIT[dtype]} of {np.abs(exact).max()}"
@@ -54,14 +61,15 @@ def test_sums_that_fp32_holds_are_exact(dtype, n, zeros, group):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kernel,dtype", [(0, F16), (1, F16), (2, F16), (3, F16), (2, BF16), (3, BF16)])
-def test_sums_that_fp32_holds_are_exact_in_every_kernel(kernel, dtype):
+@pytest.mark.parametrize("elements", ["many", "few"])
+def test_sums_that_fp32_holds_are_exact_in_every_kernel(elements, kernel, dtype):
     """Each of the kernels that a call with more than 32 columns may be given."""
     f = api.lib().mmbo_internal_gemm_w4
     f.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_size_t] * 4 + [ctypes.c_void_p] * 6
     for group, zeros in ((32, True), (64, False), (128, True)):
         m, n, k = 170, 140, 250
-        w, b, exact = _problem(dtype, m, n, k, group, zeros)
-        w.scales[:] = UNIT[dtype]
+        w, b, exact = _problem(dtype, m, n, k, group, zeros, elements)
+        w.scales[:] = UNIT[dtype] / ELEMENTS[elements][2]
         want = _rounded(UNIT[dtype] * exact, dtype)
         q, s, z, db = w.q.cuda(), w.scales.cuda(), w.zeros.cuda() if zeros else None, b.cuda()
         dc = torch.full((n, m), float("nan"), dtype=R.TORCH[dtype], device="cuda")
