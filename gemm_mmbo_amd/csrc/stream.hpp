@@ -11,8 +11,9 @@
 // 4-bit weights: a block is 128 places, half a line of a row (whole lines took longer: 28672 x 1 x 8192 33 us, with half of them 28).  Eight codes become numbers by moving nibbles to where a mantissa ends:
 //   fp16: a subnormal number, code * 2^-24, of which a packed fma makes (code - zero) * 2^-10: 11 instructions.  Not the subnormal numbers themselves: an MFMA lines its
 //     products up by the operands' exponents, which are then 10 to 13 above the products, and cuts off what fp32 would hold (one in twenty of a product's results was another fp16 number).
-//   bf16: 128 + code, the largest such number with 4 free bits: 9 instructions.  One MFMA against ones sums the columns' elements of a group; (zero point + 128) times that
-//     comes off the group's sums.
+//   bf16: a byte of 0 .. 15 is that many 2^-9 in e4m3, of which the conversion with a scale makes the code, exact: 9 instructions.  A second MFMA behind each one
+//     takes zero * column off, 32 places at a time.  (Exact code - zero as in w4_tile.hpp, 19 instructions and no second MFMA: 28672 x 1 x 8192 38.0 us for 34.7,
+//     8192 x 1 x 8192 11.5 for 10.0.  Not 128 + code and zero + 128 off the group's sums: those take bits from what is left.)
 // A group's sums are multiplied by its scale, in fp32.
 // 16-bit weights: a block is 64 places, a line of a row.
 //
@@ -73,11 +74,11 @@ __device__ inline u32x4 load32_codes(const uint8_t *p, int64_t here)
     return u.v;
 }
 
-// Eight numbers from a dword of codes.  Number n stands for (n / kUnit - kBias) + kLessZero * zero.
+// Eight numbers from a dword of codes, exact: kUnit times the code, less the zero point or not.
 template <typename T> struct Codes;
 template <> struct Codes<half_t> {
     static constexpr bool kLessZero = true;
-    static constexpr float kBias = 0.0f, kUnit = 0x1p-10f;
+    static constexpr float kUnit = 0x1p-10f;
     typedef f16x2 Zero;
     __device__ static inline Zero zero_of(uint32_t z)
     {
@@ -97,32 +98,26 @@ template <> struct Codes<half_t> {
 };
 template <> struct Codes<bf16_t> {
     static constexpr bool kLessZero = false;
-    static constexpr float kBias = 128.0f, kUnit = 1.0f;
-    // (in registers: with both constants in the instruction it would be two)
-    struct Zero { uint32_t keep, exponent; };
-    __device__ static inline Zero zero_of(uint32_t)
+    static constexpr float kUnit = 1.0f;
+    typedef bf16x8 Zero;                                // what comes off, as a second operand
+    __device__ static inline Zero zero_of(uint32_t z)
     {
-        Zero m{0x000F000Fu, 0x43004300u};
-        asm("" : "+s"(m.keep));
-        asm("" : "+v"(m.exponent));
-        return m;
+        const bf16_t v = (bf16_t)-(float)z;
+        return Zero{v, v, v, v, v, v, v, v};
     }
-    __device__ static inline bf16x8 expand(uint32_t x, const Zero &m)
+    __device__ static inline bf16x8 expand(uint32_t x, const Zero &)
     {
-        union { uint32_t d[4]; bf16x8 v; } u;
-        const uint32_t odd = x >> 4;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) u.d[p] = (__builtin_amdgcn_perm(odd, x, 0x0c040c00u + p * 0x00010001u) & m.keep) | m.exponent;
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        union { bf16x2 h[4]; bf16x8 v; } u;
+        const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
+        const uint32_t low = __builtin_amdgcn_perm(odd, even, 0x05010400u), high = __builtin_amdgcn_perm(odd, even, 0x07030602u);   // codes 0 .. 3, 4 .. 7
+        u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, 0x1p9f, false);
+        u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, 0x1p9f, true);
+        u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 0x1p9f, false);
+        u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 0x1p9f, true);
         return u.v;
     }
 };
-
-template <typename T>
-__device__ inline typename Type<T>::Frag ones()
-{
-    const uint32_t one = __is_same(T, half_t) ? 0x3C003C00u : 0x3F803F80u;
-    return frag_of<T>(u32x4{one, one, one, one});
-}
 
 // 16 bytes a lane from `p` to LDS at lds_addr + 16 * lane; 2 bytes or 1, as a dword, to lds_addr + 4 * lane (lanes that take no part leave theirs as it
 // is).  As ring::direct_load16, but from an address a lane: rows may lie anywhere.  (The instruction's offset counts for both places.)
@@ -366,43 +361,30 @@ struct Stream {
 #pragma unroll
             for (int q = 0; q < FOLDS; ++q) {
                 Sums part;
-                f32x4 sums[NT];                  // of the columns' elements
-                uint32_t z[FT];
                 Zero zero[FT];
                 clear(part);
 #pragma unroll
-                for (int c = 0; c < NT; ++c) sums[c] = f32x4{0, 0, 0, 0};
+                for (int f = 0; f < FT; ++f) zero[f] = Codes<T>::zero_of(ZEROS ? o.zeros[q][f] & kW4ZeroMask : (uint32_t)kW4Zero);
 #pragma unroll
-                for (int f = 0; f < FT; ++f) {
-                    z[f] = ZEROS ? o.zeros[q][f] & kW4ZeroMask : (uint32_t)kW4Zero;
-                    zero[f] = Codes<T>::zero_of(z[f]);
-                }
-#pragma unroll
-                for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i) {
-                    if constexpr (!Codes<T>::kLessZero)
-#pragma unroll
-                        for (int c = 0; c < NT; ++c)
-#pragma unroll
-                            for (int e = 0; e < PLANES; ++e) sums[c] = Type<T>::mfma(o.x[e][i][c], ones<T>(), sums[c]);
+                for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i)
 #pragma unroll
                     for (int f = 0; f < FT; ++f) {
                         const Frag w = Codes<T>::expand(o.codes[i][f], zero[f]);
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
-                            for (int e = 0; e < PLANES; ++e) part[c][f] = Type<T>::mfma(o.x[e][i][c], w, part[c][f]);
+                            for (int e = 0; e < PLANES; ++e) {
+                                part[c][f] = Type<T>::mfma(o.x[e][i][c], w, part[c][f]);
+                                if constexpr (!Codes<T>::kLessZero) part[c][f] = Type<T>::mfma(o.x[e][i][c], zero[f], part[c][f]);
+                            }
                     }
-                }
 #pragma unroll
                 for (int f = 0; f < FT; ++f) {
-                    // the scale of a number, and the number that stands for 0
                     const float s = (float)__builtin_bit_cast(T, (uint16_t)o.scales[q][f]) * (1.0f / Codes<T>::kUnit);
-                    const float n0 = Codes<T>::kLessZero ? 0.0f : (float)z[f] + Codes<T>::kBias;
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[c][f][r] = __builtin_fmaf(s, Codes<T>::kLessZero ? part[c][f][r] : __builtin_fmaf(-n0, sums[c][r], part[c][f][r]), acc[c][f][r]);
+                        for (int r = 0; r < 4; ++r) acc[c][f][r] = __builtin_fmaf(s, part[c][f][r], acc[c][f][r]);
                 }
             }
         } else {

@@ -191,11 +191,11 @@ size_t mmbo_static_workspace_bytes(void);
  * Dimensions and leading dimensions are at most 2^31 - 1. */
 
 /* C = alpha * W * B + beta * C: C(i, j) = alpha * sum_l W(l, i) * B[l + j*ldb] + beta * C[i + j*ldc], i < m, j < n, l < k; B and C of type
- * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  The products are summed in fp32, a group's sum is
- * multiplied by its scale in fp32, and one rounding to dtype follows at the store.  Any n: one column (a token of a
+ * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  (code - zero) * B is summed in fp32 over up to 128 places
+ * of a group, such a sum is multiplied by its scale in fp32, and one rounding to dtype follows at the store.  Any n: one column (a token of a
  * decoding step) to thousands (a prompt).  The sum's order hangs on sizes, types and n alone: the same call gives the same bits.
- * An infinity or a NaN in a column of B makes that column's results infinite or NaN (so do, in bf16, elements beyond 2^119); it
- * reaches no other column. */
+ * An infinity or a NaN in a column of B makes that column's results infinite or NaN (so may, in bf16, a group's sum beyond fp32's
+ * range before its scale: not where elements stay below 2^114, whatever the codes); it reaches no other column. */
 int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const void *alpha, const void *Q, size_t ldq,
                  const void *scales, size_t lds, const unsigned char *zeros, size_t ldz, const void *B, size_t ldb,
                  const void *beta, void *C, size_t ldc, void *stream);

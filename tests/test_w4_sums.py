@@ -43,7 +43,7 @@ def _rounded(v, dtype):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("n", [1, 3, 16, 32, 40, 150])
-@pytest.mark.parametrize("dtype", [F16])
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("elements", ["many", "few"])
 def test_sums_that_fp32_holds_are_exact(elements, dtype, n, zeros, group):
     """C takes off what the type has of the result, and the lowest bits remain."""
@@ -60,9 +60,10 @@ def test_sums_that_fp32_holds_are_exact(elements, dtype, n, zeros, group):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kernel,dtype", [(0, F16), (1, F16), (2, F16), (3, F16), (2, BF16), (3, BF16)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel", [0, 1, 2, 3])
 @pytest.mark.parametrize("elements", ["many", "few"])
-def test_sums_that_fp32_holds_are_exact_in_every_kernel(elements, kernel, dtype):
+def test_sums_that_fp32_holds_are_exact_in_every_kernel(elements, dtype, kernel):
     """Each of the kernels that a call with more than 32 columns may be given."""
     f = api.lib().mmbo_internal_gemm_w4
     f.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_size_t] * 4 + [ctypes.c_void_p] * 6
@@ -78,3 +79,28 @@ def test_sums_that_fp32_holds_are_exact_in_every_kernel(elements, kernel, dtype)
         torch.cuda.synchronize()
         off = dc.cpu().double().numpy() - want
         assert not off.any(), f"groups of {group}: {np.mean(off != 0):.2g} of all, by up to {np.abs(off).max() / UNIT[dtype]}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 16, 32, 40, 150])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_bf16_elements_up_to_2_to_the_114(n, zeros):
+    """Sums of 128 places stay below 127 * 128 * 2^114 < 2^128.  With elements near that, codes near their zero points and small scales: results far below fp32's end."""
+    m, k, group = 40, 384, 128
+    g = torch.Generator().manual_seed(n)
+    w = R.Weight(g, BF16, m, k, group, zeros)
+    w.scales[:] = 2.0 ** -10
+    code = torch.randint(7, 11, (m, k), generator=g)
+    if zeros:
+        w.zeros[:] = torch.randint(6, 12, w.zeros.shape, generator=g, dtype=torch.uint8)
+        w.zeros[::5] = 127                                          # (the farthest: every term has one sign)
+    w.q = (code[:, ::2] + 16 * code[:, 1::2]).to(torch.uint8)
+    b = (torch.randint(240, 256, (n, k), generator=g) * 2.0 ** 106).bfloat16()              # just below 2^114
+    exact, bound = R.gemm(BF16, w, b, 1.0, 0.0, None)
+    q, s, z, db = w.q.cuda(), w.scales.cuda(), w.zeros.cuda() if zeros else None, b.cuda()
+    dc = torch.empty((n, m), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    G.gemm_w4(BF16, m, n, k, group, 1.0, q, w.ldq, s, w.lds, z, w.lds, db, k, 0.0, dc, m)
+    torch.cuda.synchronize()
+    got = dc.cpu().double().numpy()
+    assert np.isfinite(got).all() and (np.abs(got - exact) <= bound).all()
