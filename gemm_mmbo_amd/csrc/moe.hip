@@ -11,6 +11,14 @@ namespace {
 
 constexpr uint32_t kTokens = 64;                // worked on at a time: a row of the grids
 
+// h between the two products is fp32, in bf16 numbers that add up to it: 8 of its 24 bits each, with its range (two numbers of the layer's type held 16 bits in bf16,
+// and in fp16 nothing above 65504 and less and less below 2^-13).  They lie in three planes; for 16 columns of 16-bit weights it lies as it is (kWhole), eight places at a time, four
+// of them in the first plane and four in the second, and is taken apart behind LDS.
+// A third less comes through a CU that way, for 44 vector instructions to 32 places, which 16 rows of 16-bit weights leave room for and 4-bit ones do not: 512 tokens, 8 of 64 experts of
+// 2048 x 1024 1,133 us, in planes 1,236; 64 tokens, 2 of 16 experts of 4096 x 2048 in 4 bits 115 us, in planes 101.
+constexpr int kPlanes = 3;
+template <bool W4, int N2> constexpr bool kWhole = N2 > 4 && !W4;
+
 struct MoeMatrix {
     W4Matrix w4;                                // 4-bit weights; of 16-bit ones w4.q is their address and w4.ldq their bytes from row to row
     int64_t stride, stride_scales, stride_zeros;    // bytes, groups, groups from expert to expert
@@ -22,7 +30,7 @@ struct MoeArgs {
     const float *bias;
     void *y;
     double *logits;                             // [tokens][experts]
-    void *h;                                    // [2][tokens * top_k][ld_h], of the layer's type
+    bf16_t *h;                                  // [plane][tokens * top_k][ld_h]
     char *table;                                // of each row of tokens
     float *parts;                               // sums of work-groups that share a tile of y: [row of tokens][tile][sharer][token][element]
     uint32_t *arrived;                          // how many of them are done: [row of tokens][tile]
@@ -398,8 +406,7 @@ __device__ inline void scale_row(Job &j, int f, const MoeMatrix &m, uint32_t exp
 }
 
 // A unit of work: h of one job, 16 of its elements: 16 rows of gate and the same of up, `hidden` shared by the wavefronts.  A work-group takes a run of units, one
-// behind the other without a pause in its loads: the wavefronts meet once a unit, over two sets of sums in turn.  h = silu(gate) * up stays fp32 as two numbers of the
-// layer's type, the second what the first leaves: in one it would carry a rounding that the definition does not have.
+// behind the other without a pause in its loads: the wavefronts meet once a unit, over two sets of sums in turn.
 // Bound by the weights' stream, and before that by the selection where it makes that itself (8 us): 8 tokens of 2048 x 1024 in 4 bits, 42 of 64 experts' 88 MB, 36 us
 // with the selection of 8; 1 token in bf16, 67 MB, 20 us.  Requests of scales, a line a row, are two fifths of all.
 template <typename T, bool W4, int N2, int FOLD, bool ZEROS, int DEPTH>
@@ -468,13 +475,22 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
         const uint32_t job = (unit0 + u) / tiles, row0 = (unit0 + u) % tiles * 16, first = table.first[job], columns = table.first[job + 1] - first;
         for (uint32_t at = threadIdx.x; at < N2 * 16; at += blockDim.x) {
             const uint32_t i = row0 + (at & 15), col = at >> 4;
-            if (i >= a.inner || col >= columns) continue;
+            if (i >= (kWhole<W4, N2> ? (a.inner + 7) / 8 * 8 : a.inner) || col >= columns) continue;
             const float g = S::total(set, 0, at & 15, col, waves), up = S::total(set, 1, at & 15, col, waves);
-            const float h = g / (1.0f + expf(-g)) * up;
-            T *const to = static_cast<T *>(a.h) + ((uint64_t)token0 * a.top_k + table.pair[first + col]) * a.ld_h + i;
-            const T high = (T)h;
-            *to = high;
-            to[(uint64_t)a.tokens * a.top_k * a.ld_h] = (T)(h - (float)high);
+            float h = g / (1.0f + expf(-g)) * up;
+            bf16_t *to = a.h + ((uint64_t)token0 * a.top_k + table.pair[first + col]) * a.ld_h;
+            const uint64_t plane = (uint64_t)a.tokens * a.top_k * a.ld_h;
+            if constexpr (kWhole<W4, N2>) {
+                reinterpret_cast<float *>(to + (i / 4 & 1) * plane + i / 8 * 8)[i % 4] = i < a.inner ? h : 0.0f;        // (whole eights are loaded)
+            } else {
+                to += i;
+#pragma unroll
+                for (int p = 0; p < kPlanes; ++p, to += plane) {
+                    const float part = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, h) & 0xFFFF0000u);     // (cut off, not rounded: no infinity comes of it)
+                    *to = (bf16_t)part;
+                    h = __builtin_isfinite(h) ? h - part : 0.0f;
+                }
+            }
         }
     };
     const uint32_t blocks = S::blocks_of(a.hidden), each = blocks / waves, more = blocks % waves, mine = each + (wave < more);
@@ -488,17 +504,28 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_gate_up_kernel(const MoeAr
     }
 }
 
+// The stream of the second product.  Planes of up to four columns stand beside them as columns of their own, which the MFMAs have room for: plane p of column c is column
+// c + p * N2.  Exact code - zero, as the MFMAs are not what bounds it.
+template <typename T, bool W4, int N2, int FT, int FOLD, bool ZEROS, int DEPTH>
+struct DownStream {
+    static constexpr bool SIDE = N2 <= 4;
+    static constexpr int PLANES = SIDE ? 1 : kWhole<W4, N2> ? 2 : kPlanes;
+    typedef stream::Stream<T, W4, SIDE ? 4 * N2 : N2, FT, PLANES, FOLD, ZEROS, DEPTH, bf16_t, true, kWhole<W4, N2>> S;
+};
+
 // A work-group: 16 * FT elements of y of its tokens: the same rows of down of every expert that was selected, the jobs' blocks one behind the other and shared
 // by the wavefronts.  What a wavefront has of a job goes to its own sums of all tokens; those are added in the order of the wavefronts.
 // Where that is too few work-groups for the chip, several (the grid's z) share the blocks: each leaves its sums in memory, and the one that is done last adds
 // them up, in the order of their numbers.  The counters that tell it were cleared by the kernel before.
-// Bound by the weights' stream and, in 4 bits, by h beside it (4 columns in two planes are 2 KB to a KB of weights): 8 tokens of 2048 x 1024, 44 MB in 20.7 us; 1 token in
+// Bound by the weights' stream and, in 4 bits, by h beside it (4 columns in three planes are 3 KB to a KB of weights): 8 tokens of 2048 x 1024, 44 MB in 20.7 us; 1 token in
 // bf16, 34 MB in 10.2 us.  Tiles of 32 rows: 21.4 and 14.9 us; twice as many work-groups to a tile: 24.0 and 10.7.
 template <typename T, bool W4, int N2, int FT, int FOLD, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs a)
 {
     using namespace stream;
-    typedef Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> S;
+    typedef DownStream<T, W4, N2, FT, FOLD, ZEROS, DEPTH> Down;
+    typedef typename Down::S S;
+    constexpr bool SIDE = Down::SIDE;
     constexpr int NT = S::NT, ROWS = 16 * FT;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63;
@@ -519,27 +546,37 @@ __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs 
         }
 #pragma unroll
         for (int q = 0; q < S::XP; ++q) {
-            const uint32_t col = S::load_column(lane, q);
-            j.x_here[q] = col < columns;
-            const T *h = static_cast<const T *>(a.h) + ((uint64_t)token0 * a.top_k + table.pair[first + min(col, columns - 1)]) * a.ld_h;
-            j.x[0][q] = h;
-            j.x[1][q] = h + (uint64_t)a.tokens * a.top_k * a.ld_h;
+            const uint32_t loaded = S::load_column(lane, q), col = SIDE ? loaded % N2 : loaded, plane = SIDE ? loaded / N2 : 0;
+            j.x_here[q] = col < columns && plane < kPlanes;
+            const uint64_t planes = (uint64_t)a.tokens * a.top_k * a.ld_h;
+            const bf16_t *h = a.h + ((uint64_t)token0 * a.top_k + table.pair[first + min(col, columns - 1)]) * a.ld_h + min(plane, (uint32_t)kPlanes - 1) * planes;
+#pragma unroll
+            for (int p = 0; p < Down::PLANES; ++p) j.x[p][q] = h + p * planes;
         }
     };
     auto flush = [&](uint32_t job, const typename S::Sums &acc) {
         const uint32_t first = table.first[job], columns = table.first[job + 1] - first;
+        auto add = [&](uint32_t col, int f, float v) { mine[table.pair[first + col] / a.top_k * ROWS + f * 16 + (lane & 15)] += table.weight[first + col] * v; };
+        if constexpr (SIDE) {                    // the planes' sums, smallest first: of one column those of a lane, of four the same lane's of each row of 16
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
+            for (int f = 0; f < FT; ++f)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t col = c * 16 + (lane >> 4) * 4 + r;
-                if (col < columns) {
-                    const float w = table.weight[first + col];
-                    float *const to = mine + table.pair[first + col] / a.top_k * ROWS + (lane & 15);
-#pragma unroll
-                    for (int f = 0; f < FT; ++f) to[f * 16] += w * acc[c][f][r];
+                for (int r = 0; r < N2; ++r) {
+                    const float v = N2 == 1 ? acc[0][f][2] + acc[0][f][1] + acc[0][f][0]
+                                            : __shfl(acc[0][f][r], lane % 16 + 32) + __shfl(acc[0][f][r], lane % 16 + 16) + acc[0][f][r];
+                    if (lane < 16 && (uint32_t)r < columns) add(r, f, v);
                 }
-            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t col = c * 16 + (lane >> 4) * 4 + r;
+                    if (col < columns)
+#pragma unroll
+                        for (int f = 0; f < FT; ++f) add(col, f, acc[c][f][r]);
+                }
+        }
     };
     const uint32_t per_job = S::blocks_of(a.inner);
     S s(a.inner, a.group / kW4Group, 0, per_job, lds + wave * S::LDS_BYTES, lane);
@@ -618,11 +655,14 @@ uint32_t most_jobs_of(const mmbo_moe_layer &l, size_t tokens)
     return std::min<uint32_t>(pairs, (uint32_t)l.experts + pairs / columns_of(l, tokens));
 }
 
+// Rows of y to a tile, / 16.  16 columns of h in three planes are 12 KB to a KB of 4-bit weights, in tiles of 32 rows 6: 64 tokens, 2 of 16 experts of 4096 x 2048 101 us, in tiles
+// of 16 rows 108; 32 tokens, 8 of 64 of 2048 x 1024 107 and 118; 20 tokens, 4 of 12 of 1000 x 2000 61 and 58.
+constexpr int down_ft(bool w4, uint32_t columns) { return w4 && columns == 16 ? 2 : 1; }
+size_t down_rows(const mmbo_moe_layer &l, size_t tokens) { return 16 * down_ft(l.group != 0, columns_of(l, tokens)); }
 // Work-groups that share a tile of y: as many as make one for each of 256 CUs, up to eight.
-constexpr size_t kDownRows = 16;
 uint32_t sharers_of(const mmbo_moe_layer &l, size_t tokens)
 {
-    const size_t tiles = ceil_div(l.hidden, kDownRows) * ceil_div(tokens, kTokens);
+    const size_t tiles = ceil_div(l.hidden, down_rows(l, tokens)) * ceil_div(tokens, kTokens);
     return (uint32_t)std::min<size_t>(std::max<size_t>(256 / tiles, 1), 8);
 }
 
@@ -637,14 +677,14 @@ Parts parts_of(const mmbo_moe_layer &l, size_t tokens)
     p.logits = 0;
     p.table = p.logits + lines(tokens * l.experts * sizeof(double));
     p.chosen = p.table + lines(ceil_div(tokens, kTokens) * table_bytes((uint32_t)(std::min<size_t>(tokens, kTokens) * l.top_k), most_jobs_of(l, tokens)));
-    const size_t tiles = ceil_div(l.hidden, kDownRows) * ceil_div(tokens, kTokens);
+    const size_t rows = down_rows(l, tokens), tiles = ceil_div(l.hidden, rows) * ceil_div(tokens, kTokens);
     p.chosen_weights = p.chosen + lines(tokens * l.top_k * sizeof(uint32_t));
     p.selected = p.chosen_weights + lines(tokens * l.top_k * sizeof(float));
     p.arrived = p.selected + lines(ceil_div(tokens, kTokens) * sizeof(uint32_t));
     p.parts = p.arrived + lines(tiles * sizeof(uint32_t));
     const uint32_t sharers = sharers_of(l, std::max<size_t>(tokens, 1));
-    p.h = p.parts + lines(sharers > 1 ? tiles * sharers * std::min<size_t>(tokens, kTokens) * kDownRows * sizeof(float) : 0);
-    p.all = p.h + lines(2 * tokens * l.top_k * p.ld_h * sizeof(half_t));
+    p.h = p.parts + lines(sharers > 1 ? tiles * sharers * std::min<size_t>(tokens, kTokens) * rows * sizeof(float) : 0);
+    p.all = p.h + lines(kPlanes * tokens * l.top_k * p.ld_h * sizeof(bf16_t));
     return p;
 }
 
@@ -678,8 +718,8 @@ hipError_t launch_gate_up(const MoeArgs &a, hipStream_t s)
 template <typename T, bool W4, int N2, int FOLD, bool ZEROS>
 hipError_t launch_down(const MoeArgs &a, hipStream_t s)
 {
-    constexpr int DEPTH = N2 == 1 ? 5 : N2 == 4 ? 4 : 2, FT = kDownRows / 16;
-    typedef stream::Stream<T, W4, N2, FT, 2, FOLD, ZEROS, DEPTH> S;
+    constexpr int DEPTH = N2 == 1 ? 5 : N2 == 4 ? W4 ? 3 : 4 : 2, FT = down_ft(W4, N2);
+    typedef typename DownStream<T, W4, N2, FT, FOLD, ZEROS, DEPTH>::S S;
     static std::atomic<bool> set[64];
     auto kernel = moe_down_kernel<T, W4, N2, FT, FOLD, ZEROS, DEPTH>;
     if (hipError_t e = allow_lds(kernel, set)) return e;
@@ -763,7 +803,7 @@ int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, cons
     a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy;
     a.alpha = *static_cast<const float *>(alpha); a.beta = *static_cast<const float *>(beta);
     a.logits = reinterpret_cast<double *>(ws + p.logits);
-    a.h = ws + p.h;
+    a.h = reinterpret_cast<bf16_t *>(ws + p.h);
     a.ld_h = (uint32_t)p.ld_h;
     a.table = ws + p.table;
     a.chosen = reinterpret_cast<uint32_t *>(ws + p.chosen);
@@ -771,7 +811,7 @@ int mmbo_moe(const mmbo_moe_layer *layer, size_t tokens, const void *alpha, cons
     a.selected = reinterpret_cast<uint32_t *>(ws + p.selected);
     a.arrived = reinterpret_cast<uint32_t *>(ws + p.arrived);
     a.parts = reinterpret_cast<float *>(ws + p.parts);
-    a.down_tiles = (uint32_t)ceil_div(l.hidden, kDownRows);
+    a.down_tiles = (uint32_t)ceil_div(l.hidden, down_rows(l, tokens));
     a.sharers = sharers_of(l, tokens);
     a.ids = ids;
     a.weights = weights;

@@ -12,8 +12,9 @@
 //   fp16: a subnormal number, code * 2^-24, of which a packed fma makes (code - zero) * 2^-10: 11 instructions.  Not the subnormal numbers themselves: an MFMA lines its
 //     products up by the operands' exponents, which are then 10 to 13 above the products, and cuts off what fp32 would hold (one in twenty of a product's results was another fp16 number).
 //   bf16: a byte of 0 .. 15 is that many 2^-9 in e4m3, of which the conversion with a scale makes the code, exact: 9 instructions.  A second MFMA behind each one
-//     takes zero * column off, 32 places at a time.  (Exact code - zero as in w4_tile.hpp, 19 instructions and no second MFMA: 28672 x 1 x 8192 38.0 us for 34.7,
-//     8192 x 1 x 8192 11.5 for 10.0.  Not 128 + code and zero + 128 off the group's sums: those take bits from what is left.)
+//     takes zero * column off, 32 places at a time.  Not 128 + code and zero + 128 off the group's sums: those take bits from what is left.  Or (LESS_ZERO) from the
+//     subnormal fp16 number one mixed-precision fma makes code - zero in fp32, and two of those are packed: 19 instructions and no second MFMA (28672 x 1 x 8192 38.0 us
+//     for 34.7, 8192 x 1 x 8192 11.5 for 10.0).
 // A group's sums are multiplied by its scale, in fp32.
 // 16-bit weights: a block is 64 places, a line of a row.
 //
@@ -74,9 +75,9 @@ __device__ inline u32x4 load32_codes(const uint8_t *p, int64_t here)
     return u.v;
 }
 
-// Eight numbers from a dword of codes, exact: kUnit times the code, less the zero point or not.
-template <typename T> struct Codes;
-template <> struct Codes<half_t> {
+// Eight numbers from a dword of codes, exact: kUnit times the code, less the zero point (always with LESS_ZERO) or not.
+template <typename T, bool LESS_ZERO = false> struct Codes;
+template <bool LESS_ZERO> struct Codes<half_t, LESS_ZERO> {
     static constexpr bool kLessZero = true;
     static constexpr float kUnit = 0x1p-10f;
     typedef f16x2 Zero;
@@ -96,7 +97,7 @@ template <> struct Codes<half_t> {
         return u.v;
     }
 };
-template <> struct Codes<bf16_t> {
+template <> struct Codes<bf16_t, false> {
     static constexpr bool kLessZero = false;
     static constexpr float kUnit = 1.0f;
     typedef bf16x8 Zero;                                // what comes off, as a second operand
@@ -116,6 +117,25 @@ template <> struct Codes<bf16_t> {
         u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 0x1p9f, false);
         u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 0x1p9f, true);
         return u.v;
+    }
+};
+
+template <> struct Codes<bf16_t, true> {
+    static constexpr bool kLessZero = true;
+    static constexpr float kUnit = 1.0f;
+    typedef float Zero;
+    __device__ static inline Zero zero_of(uint32_t z) { return -(float)z; }
+    __device__ static inline bf16x8 expand(uint32_t x, Zero z)
+    {
+        bf16x8 v;
+        const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(odd, even, 0x0c040c00u + p * 0x00010001u));
+            v[2 * p] = (bf16_t)__builtin_fmaf((float)h[0], 0x1p24f, z);
+            v[2 * p + 1] = (bf16_t)__builtin_fmaf((float)h[1], 0x1p24f, z);
+        }
+        return v;
     }
 };
 
@@ -149,13 +169,15 @@ __device__ inline uint32_t chunk_at(uint32_t row, uint32_t chunk)
 // The sums of a wavefront over its share of several jobs: of each job blocks block0 .. block0 + per_job - 1 of k, job after job, and of all these blocks
 // numbers first .. first + count - 1.  enter(job, Job &) says where its operands lie, flush(job, sums) takes the sums of what the wavefront had of it.  Results
 // of columns that do not exist are not defined.  lds: the wavefront's own LDS_BYTES.
-// N2: columns side by side, 1, 4, 16 or 32, each in PLANES numbers of type T, which are added.  FT: tiles of 16 rows.
+// T: of weights and scales; TX: of the columns, and what is multiplied -- with TX bf16, T may be fp16.
+// N2: columns side by side, 1, 4, 16 or 32, each in PLANES numbers of type TX, which are added.  FT: tiles of 16 rows.  LESS_ZERO: of Codes.
+// FP32: columns in fp32 in the room of two planes, four places of eight in each; the last eight are whole ones.
 // FOLD (4-bit weights): places whose sums are multiplied by a scale at once: 128 where groups are whole multiples of that, 64, else 32.
-template <typename T, bool W4, int N2, int FT, int PLANES, int FOLD, bool ZEROS, int DEPTH>
+template <typename T, bool W4, int N2, int FT, int PLANES, int FOLD, bool ZEROS, int DEPTH, typename TX = T, bool LESS_ZERO = false, bool FP32 = false>
 struct Stream {
     static_assert(N2 == 1 || N2 == 4 || N2 == 16 || N2 == 32, "");
-    typedef typename Type<T>::Frag Frag;
-    typedef typename Codes<T>::Zero Zero;
+    typedef typename Type<TX>::Frag Frag;
+    typedef typename Codes<TX, LESS_ZERO>::Zero Zero;
     static constexpr int NT = N2 > 16 ? N2 / 16 : 1, BLOCK = W4 ? 128 : 64, STEPS = BLOCK / 32, ROW_BYTES = W4 ? BLOCK / 2 : 128;
     static constexpr int FOLDS = W4 ? BLOCK / FOLD : 1;
     static constexpr int WP = ROW_BYTES / 64, W_TILE = WP * 1024;
@@ -197,7 +219,7 @@ struct Stream {
         const uint8_t *w[FT][WP];               // rows load_row(lane, 0 ..) of a tile: of codes, or of elements
         const T *scales[FT];                    // row lane % 16
         const uint8_t *zeros[FT];
-        const T *x[PLANES][XP];                 // columns load_column(lane, 0 ..)
+        const TX *x[PLANES][XP];                 // columns load_column(lane, 0 ..)
         bool x_here[XP];                        // .. exist
     };
     __device__ static inline uint32_t load_row(int lane, int p) { return ROW_BYTES == 64 ? lane >> 2 : p * 8 + (lane >> 3); }
@@ -310,7 +332,7 @@ struct Stream {
 #pragma unroll
                 for (int j = 0; j < X_LOADS; ++j)
                     if (from.x_here[j % XP]) {
-                        const int64_t here = left - x_line(lane, j) - x_chunk(lane, j % XP) * 8;
+                        const int64_t here = (left - x_line(lane, j) - x_chunk(lane, j % XP) * 8 + (FP32 ? 7 : 0)) & (FP32 ? ~7 : ~0);
                         *reinterpret_cast<u32x4 *>(slot_at + X_AT + q * X_PLANE + j * 1024 + lane * 16) = load8(from.x[q][j % XP] + x_line(0, j), here);
                     }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -336,7 +358,7 @@ struct Stream {
             for (int i = 0; i < STEPS; ++i)
 #pragma unroll
                 for (int c = 0; c < NT; ++c)
-                    o.x[q][i][c] = frag_of<T>(*reinterpret_cast<const u32x4 *>(at + X_AT + q * X_PLANE + i / 2 * N2 * 128 +
+                    o.x[q][i][c] = frag_of<TX>(*reinterpret_cast<const u32x4 *>(at + X_AT + q * X_PLANE + i / 2 * N2 * 128 +
                                                                                chunk_at<128>((lane & (N2 < 16 ? N2 - 1 : 15)) + c * 16, i % 2 * 4 + quarter)));
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
@@ -355,6 +377,29 @@ struct Stream {
         }
     }
 
+    // What the MFMAs take of tile c of columns and 32 places: its planes, or fp32 in three bf16 numbers, cut off where one ends (finite numbers exactly).
+    static constexpr int kParts = FP32 ? 3 : PLANES;
+    __device__ inline void parts(Frag (&x)[kParts], int i, int c) const
+    {
+        if constexpr (FP32) {
+            union { Frag from[2]; uint32_t u[8]; float v[8]; } h;
+            h.from[0] = o.x[0][i][c];
+            h.from[1] = o.x[1][i][c];
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                union { uint32_t d[4]; Frag v; } u;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) u.d[p] = __builtin_amdgcn_perm(h.u[2 * p + 1], h.u[2 * p], 0x07060302u);
+                x[e] = u.v;
+                if (e < 2)
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) h.v[p] -= __builtin_bit_cast(float, h.u[p] & 0xFFFF0000u);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < PLANES; ++e) x[e] = o.x[e][i][c];
+        }
+    }
     __device__ inline void multiply(Sums &acc)
     {
         if constexpr (W4) {
@@ -364,23 +409,28 @@ struct Stream {
                 Zero zero[FT];
                 clear(part);
 #pragma unroll
-                for (int f = 0; f < FT; ++f) zero[f] = Codes<T>::zero_of(ZEROS ? o.zeros[q][f] & kW4ZeroMask : (uint32_t)kW4Zero);
+                for (int f = 0; f < FT; ++f) zero[f] = Codes<TX, LESS_ZERO>::zero_of(ZEROS ? o.zeros[q][f] & kW4ZeroMask : (uint32_t)kW4Zero);
 #pragma unroll
-                for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i)
+                for (int i = q * (STEPS / FOLDS); i < (q + 1) * (STEPS / FOLDS); ++i) {
+                    Frag w[FT];
 #pragma unroll
-                    for (int f = 0; f < FT; ++f) {
-                        const Frag w = Codes<T>::expand(o.codes[i][f], zero[f]);
+                    for (int f = 0; f < FT; ++f) w[f] = Codes<TX, LESS_ZERO>::expand(o.codes[i][f], zero[f]);
 #pragma unroll
-                        for (int c = 0; c < NT; ++c)
+                    for (int c = 0; c < NT; ++c) {
+                        Frag x[kParts];
+                        parts(x, i, c);
 #pragma unroll
-                            for (int e = 0; e < PLANES; ++e) {
-                                part[c][f] = Type<T>::mfma(o.x[e][i][c], w, part[c][f]);
-                                if constexpr (!Codes<T>::kLessZero) part[c][f] = Type<T>::mfma(o.x[e][i][c], zero[f], part[c][f]);
+                        for (int f = 0; f < FT; ++f)
+#pragma unroll
+                            for (int e = 0; e < kParts; ++e) {
+                                part[c][f] = Type<TX>::mfma(x[e], w[f], part[c][f]);
+                                if constexpr (!Codes<TX, LESS_ZERO>::kLessZero) part[c][f] = Type<TX>::mfma(x[e], zero[f], part[c][f]);
                             }
                     }
+                }
 #pragma unroll
                 for (int f = 0; f < FT; ++f) {
-                    const float s = (float)__builtin_bit_cast(T, (uint16_t)o.scales[q][f]) * (1.0f / Codes<T>::kUnit);
+                    const float s = (float)__builtin_bit_cast(T, (uint16_t)o.scales[q][f]) * (1.0f / Codes<TX, LESS_ZERO>::kUnit);
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -391,11 +441,34 @@ struct Stream {
 #pragma unroll
             for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-                for (int f = 0; f < FT; ++f)
+                for (int c = 0; c < NT; ++c) {
+                    Frag x[kParts];
+                    parts(x, i, c);
 #pragma unroll
-                    for (int c = 0; c < NT; ++c)
+                    for (int f = 0; f < FT; ++f) {
+                        Frag w[kWeightPlanes];
+                        weights(w, o.w[i][f]);
 #pragma unroll
-                        for (int e = 0; e < PLANES; ++e) acc[c][f] = Type<T>::mfma(o.x[e][i][c], frag_of<T>(o.w[i][f]), acc[c][f]);
+                        for (int e = 0; e < kParts; ++e)
+#pragma unroll
+                            for (int p = 0; p < kWeightPlanes; ++p) acc[c][f] = Type<TX>::mfma(x[e], w[p], acc[c][f]);
+                    }
+                }
+        }
+    }
+    // Weights of 16 bits as second operands: as they are, or fp16 in two bf16 numbers, 8 and 3 bits of its 11 (finite numbers exactly).
+    static constexpr int kWeightPlanes = __is_same(T, TX) ? 1 : 2;
+    __device__ static inline void weights(Frag (&w)[kWeightPlanes], u32x4 v)
+    {
+        if constexpr (kWeightPlanes == 1) {
+            w[0] = frag_of<TX>(v);
+        } else {
+            const f16x8 high = frag_of<T>(v & 0xFFF8FFF8u), low = frag_of<T>(v) - high;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[0][i] = (TX)(float)high[i];
+                w[1][i] = (TX)(float)low[i];
+            }
         }
     }
     __device__ static inline void clear(Sums &acc)

@@ -20,26 +20,6 @@ using namespace stream;
 
 constexpr int BLOCK = 128, STEPS = 4;
 
-template <typename T> struct Exact;
-template <> struct Exact<half_t> : Codes<half_t> {};
-template <> struct Exact<bf16_t> {
-    static constexpr float kUnit = 1.0f;
-    typedef float Zero;
-    __device__ static inline Zero zero_of(uint32_t z) { return -(float)z; }
-    __device__ static inline bf16x8 expand(uint32_t x, Zero z)
-    {
-        bf16x8 v;
-        const uint32_t even = x & 0x0F0F0F0Fu, odd = x >> 4 & 0x0F0F0F0Fu;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(odd, even, 0x0c040c00u + p * 0x00010001u));
-            v[2 * p] = (bf16_t)__builtin_fmaf((float)h[0], 0x1p24f, z);
-            v[2 * p + 1] = (bf16_t)__builtin_fmaf((float)h[1], 0x1p24f, z);
-        }
-        return v;
-    }
-};
-
 template <typename T, int WM, int NC, int FOLDS, bool ZEROS, int DEPTH>
 struct Config {
     static constexpr int ROWS = 32 * WM, COLUMNS = 16 * NC, THREADS = 64 * WM;
@@ -151,11 +131,11 @@ gemm_w4_tile_kernel(const GemmW4Args a)
 #pragma unroll
         for (int q = 0; q < FOLDS; ++q) {
             float scale[2];
-            typename Exact<T>::Zero zero[2];
+            typename Codes<T, true>::Zero zero[2];
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
-                scale[f] = (float)__builtin_bit_cast(T, *reinterpret_cast<const uint16_t *>(at + C::S_AT + (wave * 2 + f) * C::S_TILE + (q * 16 + row) * 4)) * (1.0f / Exact<T>::kUnit);
-                zero[f] = Exact<T>::zero_of(ZEROS ? *reinterpret_cast<const uint32_t *>(at + C::Z_AT + (wave * 2 + f) * C::S_TILE + (q * 16 + row) * 4) & kW4ZeroMask : (uint32_t)kW4Zero);
+                scale[f] = (float)__builtin_bit_cast(T, *reinterpret_cast<const uint16_t *>(at + C::S_AT + (wave * 2 + f) * C::S_TILE + (q * 16 + row) * 4)) * (1.0f / Codes<T, true>::kUnit);
+                zero[f] = Codes<T, true>::zero_of(ZEROS ? *reinterpret_cast<const uint32_t *>(at + C::Z_AT + (wave * 2 + f) * C::S_TILE + (q * 16 + row) * 4) & kW4ZeroMask : (uint32_t)kW4Zero);
             }
             f32x4 part[2][NC];
 #pragma unroll
@@ -167,7 +147,7 @@ gemm_w4_tile_kernel(const GemmW4Args a)
                 Frag wf[2];
 #pragma unroll
                 for (int f = 0; f < 2; ++f)
-                    wf[f] = Exact<T>::expand(*reinterpret_cast<const uint32_t *>(at + C::W_AT + (wave * 2 + f) * 1024 + chunk_at<64>(row, i) + quarter * 4), zero[f]);
+                    wf[f] = Codes<T, true>::expand(*reinterpret_cast<const uint32_t *>(at + C::W_AT + (wave * 2 + f) * 1024 + chunk_at<64>(row, i) + quarter * 4), zero[f]);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const Frag xf = frag_of<T>(*reinterpret_cast<const u32x4 *>(at + (i / 2 * NC + c) * 2048 + chunk_at<128>(row, i % 2 * 4 + quarter)));

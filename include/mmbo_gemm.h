@@ -191,9 +191,10 @@ size_t mmbo_static_workspace_bytes(void);
  * Dimensions and leading dimensions are at most 2^31 - 1. */
 
 /* C = alpha * W * B + beta * C: C(i, j) = alpha * sum_l W(l, i) * B[l + j*ldb] + beta * C[i + j*ldc], i < m, j < n, l < k; B and C of type
- * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  (code - zero) * B is summed in fp32 over up to 128 places
- * of a group, such a sum is multiplied by its scale in fp32, and one rounding to dtype follows at the store.  Any n: one column (a token of a
- * decoding step) to thousands (a prompt).  The sum's order hangs on sizes, types and n alone: the same call gives the same bits.
+ * dtype, alpha and beta host pointers to float.  beta == 0: C is not read.  (code - zero) * B is summed in fp32 over up to 128 places of
+ * a group (in bf16, code * B and zero * B apart for 32 of them at a time), such a sum is multiplied by its scale in fp32, and one
+ * rounding to dtype follows at the store.  Any n: one column (a token of a decoding step) to thousands (a prompt).  The sum's order
+ * hangs on sizes, types and n alone: the same call gives the same bits.
  * An infinity or a NaN in a column of B makes that column's results infinite or NaN (so may, in bf16, a group's sum beyond fp32's
  * range before its scale: not where elements stay below 2^114, whatever the codes); it reaches no other column. */
 int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, size_t group, const void *alpha, const void *Q, size_t ldq,
@@ -228,7 +229,7 @@ int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *
  * down has `hidden` rows and `inner` columns; both row by row (k contiguous).  group == 0: elements of type dtype, data[l + i*ld +
  * e*stride]; otherwise 4-bit weights in the format above with that group: code (l, i) of expert e is code number l + i*ld + e*stride (both even),
  * its scale scales[g + i*lds + e*stride_scales], its zero point zeros[g + i*ldz + e*stride_zeros] (zeros NULL: 8).
- * h is held as the sum of two numbers of type dtype (an h beyond that type's range is infinite), every sum in fp32. */
+ * h is held in fp32, with its range, whatever dtype is, and so is every sum; what an infinite h or weight enters becomes infinite or NaN. */
 #define MMBO_MOE_SOFTMAX 0
 #define MMBO_MOE_SIGMOID 1
 #define MMBO_MOE_MAX_TOKENS 512
