@@ -223,6 +223,8 @@ int mmbo_w4_dequantize(int dtype, size_t m, size_t k, size_t group, const void *
  *   selected: the top_k experts with the largest logit -- with a bias: the largest score + bias[e] --, ties to the lower index,
  *       NaN behind everything else
  *   weight = score, or (renormalize) score over the sum of the selected scores; 0 where that sum is 0
+ *       (a NaN among a token's logits makes all scores of its softmax NaN, but where they count against each other alone --
+ *       renormalize without a bias -- only that expert's)
  *   h = silu(gate * x) * (up * x), silu(v) = v / (1 + exp(-v));  y = alpha * sum over the selected of weight * (down * h) + beta * y
  *
  * Expert e's gate and up are rows 0 .. inner-1 and inner .. 2*inner-1 of one matrix of 2*inner rows and `hidden` columns, gate_up;
