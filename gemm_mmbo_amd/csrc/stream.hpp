@@ -8,7 +8,7 @@
 // no register for what is under way.  Loads have to come as whole memory lines: with a lane to a row, as MFMAs want them, a CU got 11 bytes a clock
 // (4096 x 16 x 14336 in 4 bits: 24 us), with 64 bytes to four lanes 20 (13.3 us), though halves of a line were asked for one behind the other.
 //
-// 4-bit weights: a block is 128 places, half a line of a row (whole lines took longer: 28672 x 1 x 8192 33 us, with half of them 28).  Eight codes become numbers by moving nibbles to where a mantissa ends:
+// 4-bit weights: a block is 128 places, half a line of a row (whole lines took a sixth longer with one column: 33 us for 28, before scales went through the ring).  Eight codes become numbers by moving nibbles to where a mantissa ends:
 //   fp16: a subnormal number, code * 2^-24, of which a packed fma makes (code - zero) * 2^-10: 11 instructions.  Not the subnormal numbers themselves: an MFMA lines its
 //     products up by the operands' exponents, which are then 10 to 13 above the products, and cuts off what fp32 would hold (one in twenty of a product's results was another fp16 number).
 //   bf16: a byte of 0 .. 15 is that many 2^-9 in e4m3, of which the conversion with a scale makes the code, exact: 9 instructions.  A second MFMA behind each one
@@ -18,9 +18,9 @@
 // A group's sums are multiplied by its scale, in fp32.
 // 16-bit weights: a block is 64 places, a line of a row.
 //
-// What bounds it: one column, the weights from memory beside requests of scales, a line a row and block (28672 x 1 x 8192: fp16 31 us, bf16 with zero points 35, 121 MB
-// take 21; 4096 x 1 x 4096 4.9 us, a launch).  More columns, what a CU gets from the L2, some 50 bytes a ns: each work-group reads all columns for its 16 or 32 rows
-// (4096 x 16 x 14336 12.9 us for 0.6 MB a CU, 8192 x 64 x 8192 27.1 for 1.3 MB).
+// What bounds it: one column, the weights from memory beside requests of scales, a line a row and block (28672 x 1 x 8192: 31.6 us in either type, with zero points 34.7, for
+// 119 and 121 MB, which take 21; 4096 x 1 x 4096 5.0 us, a launch).  More columns, what a CU gets from the L2, some 50 bytes a ns: each work-group reads all columns for its 16
+// or 32 rows (4096 x 16 x 14336 12.9 us for 0.6 MB a CU, 8192 x 64 x 8192 26.5 for 1.3 MB).
 #pragma once
 
 #include <type_traits>

@@ -41,7 +41,8 @@ __device__ inline float nearest(float w, float s, float by)
 
 // Sixteen bytes or the elements of them that exist (any number); the others are 0.
 template <typename TW> constexpr int kPer16 = 16 / (int)sizeof(TW);
-typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+using stream::u32x4_any;
+using stream::u32_any;
 template <typename TW>
 __device__ inline u32x4 load_part(const TW *p, int64_t here)
 {
@@ -149,7 +150,6 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const QuantArgs a)
                 codes = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(c1, 16.0f, c0), e / 2, codes);
             }
             const uint32_t here = min(length - l, (uint32_t)E);
-            typedef uint32_t __attribute__((aligned(1))) u32_any;
             typedef uint16_t __attribute__((aligned(1))) u16_any;
             if (here == E) {
                 if constexpr (E == 8) *reinterpret_cast<u32_any *>(q + l / 2) = codes;
@@ -177,7 +177,6 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const QuantArgs a)
     const uint8_t *q = a.w.q + i * a.w.ldq + l / 2;
     T *to = static_cast<T *>(a.W) + i * a.ldw + l;
     union { u32x4 v; T e[8]; } u;
-    typedef uint32_t __attribute__((aligned(1))) u32_any;
     if (l + 8 <= a.k) {
         const uint32_t codes = *reinterpret_cast<const u32_any *>(q);
 #pragma unroll
@@ -221,8 +220,8 @@ constexpr int kStreamWaves = 8;
 template <typename T, int N2, int FT, int FOLD, bool ZEROS>
 hipError_t launch_stream_kernel(const GemmW4Args &a, hipStream_t s)
 {
-    // Blocks under way in a ring.  Work-groups beside each other on a CU hide what a deeper ring would, and need the LDS: 28672 x 1 x 8192 29.4 us
-    // with rings of 3, 33.7 in work-groups of sixteen wavefronts; 4096 x 16 x 14336 13.3 with rings of 2, 13.6 of 3, 14.5 of 4.
+    // Blocks under way in a ring.  Work-groups beside each other on a CU hide what a deeper ring would, and need the LDS: 28672 x 1 x 8192 31.5 us with rings of 2, 3 and
+    // 4 (work-groups of sixteen wavefronts took a seventh longer); rings of 2, 3 and 4: 4096 x 16 x 14336 13.5, 14.0 and 14.6 us, 8192 x 64 x 8192 27.1, 28.5 and 36.1.
     constexpr int DEPTH = N2 == 1 ? 3 : 2;
     typedef stream::Stream<T, true, N2, FT, 1, FOLD, ZEROS, DEPTH> S;
     constexpr int kWaveBytes = S::LDS_BYTES + 2 * S::SET_FLOATS * 4, kMost = std::min<int>(kStreamWaves, kLds / kWaveBytes);

@@ -7,7 +7,7 @@
 //   bf16: from the subnormal fp16 number code * 2^-24 one mixed-precision fma makes code - zero in fp32, and two of those are packed: 19.
 // A group's sums, in fp32, are multiplied by its scale and added to the total.  What bounds it is the issue of vector instructions beside the MFMAs: 16
 // MFMAs of 16 clocks a step of 32 places, and for those two wavefronts of a SIMD 2 * (38 (fp16: 22) + 16 + 16) issues of 4.
-// 8192 x 2048 x 4096 in groups of 128: fp16 137 us, bf16 147, 1.0 and 0.94 PFLOP/s; groups of 64 151 and 163, of 32 166 (fp16).
+// 8192 x 2048 x 4096 in groups of 128: fp16 136 us, bf16 147, 1.0 and 0.94 PFLOP/s; groups of 64 151 and 163, of 32 169 (fp16).
 #pragma once
 
 #include "stream.hpp"
