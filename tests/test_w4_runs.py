@@ -114,3 +114,29 @@ def test_zero_points_of_a_byte_in_a_layer(dtype, group, tokens):
     exact, bound, ids, _ = counts.exact()
     y, got_ids, _ = p.run()
     assert np.array_equal(got_ids, ids) and (np.abs(y.double().numpy() - exact) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,m,n,k", [(F16, 2 ** 22 + 37, 1, 40), (BF16, 2 ** 22 + 37, 3, 40), (F16, 2 ** 22 + 5, 40, 32), (BF16, 20, 2 ** 16 + 19, 70), (F16, 300, 2 ** 16 + 1, 33)])
+def test_more_rows_or_columns_than_one_launch_takes(dtype, m, n, k):
+    g = torch.Generator().manual_seed(n)
+    w = R.Weight(g, dtype, m, k, 32, True)
+    b = torch.randn((n, k), generator=g).to(R.TORCH[dtype])
+    c = torch.randn((n, m + 1), generator=g).to(R.TORCH[dtype])
+    exact, bound = _gemm_on_gpu(dtype, w, b, 0.5, -1.0, c[:, :m])
+    out = c.cuda()
+    q, s, z, db = w.q.cuda(), w.scales.cuda(), w.zeros.cuda(), b.cuda()
+    torch.cuda.synchronize()
+    G.gemm_w4(dtype, m, n, k, 32, 0.5, q, w.ldq, s, w.lds, z, w.lds, db, k, -1.0, out, m + 1)
+    torch.cuda.synchronize()
+    worst = ((out[:, :m].double() - exact).abs() / bound).max().item()
+    assert worst <= 1.0 and torch.equal(out[:, m].cpu(), c[:, m]), f"{worst:.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("tokens", [64, 130])
+def test_most_pairs_and_jobs(group, tokens):
+    """2048 pairs to 64 tokens, of 512 experts: the largest table, beside the fewest wavefronts."""
+    for dtype in (F16, BF16):
+        _check(Problem(dtype, tokens, 40, 24, G.MOE_MAX_EXPERTS, G.MOE_MAX_TOP_K, group, zeros=True))
