@@ -518,7 +518,7 @@ struct DownStream {
 // by the wavefronts.  What a wavefront has of a job goes to its own sums of all tokens; those are added in the order of the wavefronts.
 // Where that is too few work-groups for the chip, several (the grid's z) share the blocks: each leaves its sums in memory, and the one that is done last adds
 // them up, in the order of their numbers.  The counters that tell it were cleared by the kernel before.
-// Bound by the weights' stream and, in 4 bits, by h beside it (4 columns in three planes are 3 KB to a KB of weights): 8 tokens of 2048 x 1024, 44 MB in 22 us; 1 token in
+// Bound by the weights' stream and, in 4 bits, by h beside it (4 columns in three planes are 3 KB to a KB of weights): 8 tokens of 2048 x 1024, 44 MB in 21 us; 1 token in
 // bf16, 34 MB in 9.5 us; 64 tokens of 4096 x 2048, 268 MB in 61 us, in 4 bits 69 MB in 46.  Twice as many work-groups to a tile: 24.0 for 20.7 and 10.7 for 10.2 (h in two planes then).
 template <typename T, bool W4, int N2, int FT, int FOLD, bool ZEROS, int DEPTH>
 __global__ void __launch_bounds__(kMoeWaves * 64) moe_down_kernel(const MoeArgs a)
